@@ -352,4 +352,45 @@ int gi_rope_inplace(void* q, void* k, const void* cos_t, const void* sin_t,
                          as_stream(stream));
 }
 
+int gi_rope_rows(const void* q, void* q_out, const void* k, void* k_out, const int64_t* positions,
+                 const double* inv_freq, int dtype, int T, int Hq, int Hk, int D, int rotary_dim, int interleaved,
+                 float mscale, int64_t q_st, int64_t q_sh, int64_t qo_st, int64_t qo_sh, int64_t k_st, int64_t k_sh,
+                 int64_t ko_st, int64_t ko_sh, void* stream) {
+  const int64_t qs[2] = {q_st, q_sh}, qos[2] = {qo_st, qo_sh}, ks[2] = {k_st, k_sh}, kos[2] = {ko_st, ko_sh};
+  return gi::launch_rope_rows(q, q_out, k, k_out, positions, inv_freq, dtype, T, Hq, Hk, D, rotary_dim, interleaved,
+                              mscale, qs, qos, ks, kos, as_stream(stream));
+}
+
+int gi_kv_slots(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* block_table, int max_pages,
+                int64_t table_stride, const int32_t* free_pages, int n_free, const int32_t* free_used, int page_size,
+                int64_t* slots, int64_t* positions, int n_tokens, int32_t* q_start, int32_t* seq_lens,
+                int32_t* status, void* stream) {
+  return gi::launch_kv_slots(ctx_lens, new_lens, B, block_table, max_pages, table_stride, free_pages, n_free,
+                             free_used, page_size, slots, positions, n_tokens, q_start, seq_lens, status,
+                             as_stream(stream));
+}
+
+int gi_kv_append(const void* k, const void* v, int dtype, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                 const int64_t* slots, int T, int Hk, int D, int page_size, int64_t num_pages, void* k_cache,
+                 void* v_cache, float* k_scale, float* v_scale, void* stream) {
+  const int64_t ks[2] = {k_st, k_sh}, vs[2] = {v_st, v_sh};
+  return gi::launch_kv_append(k, v, dtype, ks, vs, slots, T, Hk, D, page_size, num_pages, k_cache, v_cache, k_scale,
+                              v_scale, as_stream(stream));
+}
+
+size_t gi_kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D) {
+  return gi::kv_attention_workspace_bytes(T, B, Hq, Hk, D);
+}
+
+int gi_kv_attention(const void* q, int dtype, int64_t q_st, int64_t q_sh, const void* k_cache, const void* v_cache,
+                    const float* k_scale, const float* v_scale, const int32_t* block_table, int max_pages,
+                    int64_t table_stride, const int32_t* seq_lens, const int32_t* q_start, void* out, int64_t o_st,
+                    int64_t o_sh, int T, int B, int Hq, int Hk, int D, int page_size, int64_t num_pages, float scale,
+                    int window, void* workspace, size_t workspace_bytes, void* stream) {
+  const int64_t qs[2] = {q_st, q_sh}, os[2] = {o_st, o_sh};
+  return gi::launch_kv_attention(q, dtype, qs, k_cache, v_cache, k_scale, v_scale, block_table, table_stride,
+                                 max_pages, seq_lens, q_start, out, os, T, B, Hq, Hk, D, page_size, num_pages, scale,
+                                 window, workspace, workspace_bytes, as_stream(stream));
+}
+
 }  // extern "C"

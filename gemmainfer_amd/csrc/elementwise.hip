@@ -91,6 +91,118 @@ __global__ __launch_bounds__(256) void rope_kernel(T* q, T* k, const T* cs, cons
   }
 }
 
+// Rotary embedding of packed rows: the pair (x1, x2) of frequency f at position
+// p becomes (x1 c - x2 s, x2 c + x1 s), c = m cos(p f), s = m sin(p f).  The
+// angle is formed in fp64 and reduced to (-1/2, 1/2] turns before it is rounded
+// to fp32: at a position of 10^6 an fp32 product would be off by up to 0.03
+// radians, a reduced one by 1e-7.  One workgroup a row: its cos and sin are
+// worked out once, into LDS, and serve every head of q and k.  Bound by HBM:
+// each element is read and written once.
+constexpr int kRopeThreads = 256;
+constexpr int kRopeMaxPairs = 512;
+
+struct RopeArgs {
+  const void* in[2];   // q, k
+  void* out[2];
+  int64_t in_st[2], in_sh[2], out_st[2], out_sh[2];  // row and head strides, elements
+  const int64_t* pos;
+  const double* freq;
+  float mscale;
+  int heads[2], D, pairs;
+};
+
+// Explicit fused steps, each rounded to fp32 (for fp16 results the compiler
+// would otherwise join the last one and the conversion here and there): every
+// form of the kernel gives the same bits.
+__device__ __forceinline__ void turn_pair(float x1, float x2, float c, float s, float& y1, float& y2) {
+  y1 = fmaf(x1, c, -(x2 * s));
+  y2 = fmaf(x2, c, x1 * s);
+  asm("" : "+v"(y1), "+v"(y2));
+}
+
+template <typename T>
+struct alignas(16) Pack8 {
+  T v[8];
+};
+
+// kVec: 8 elements of a head at a time (rows, heads and the halves 16-byte
+// aligned); otherwise one pair at a time.
+template <typename T, bool kInter, bool kVec>
+__global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs a) {
+  __shared__ float cs[kRopeMaxPairs], sn[kRopeMaxPairs];
+  const int64_t row = blockIdx.x;
+  const double p = (double)a.pos[row];
+  for (int i = threadIdx.x; i < a.pairs; i += kRopeThreads) {
+    const double turns = p * a.freq[i] * 0.15915494309189535;  // 1 / (2 pi)
+    const float r = (float)(turns - rint(turns));
+    float s, c;
+    sincospif(2.f * r, &s, &c);
+    cs[i] = c * a.mscale;
+    sn[i] = s * a.mscale;
+  }
+  __syncthreads();
+  const int R = 2 * a.pairs;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const T* in = (const T*)a.in[w] + row * a.in_st[w];
+    T* out = (T*)a.out[w] + row * a.out_st[w];
+    if (kVec) {
+      // units of a head: the rotated ones (8 pairs each where halves are apart,
+      // 4 where pairs are adjacent), then those behind them, only copied
+      const int turn = kInter ? R >> 3 : R >> 4, rest = (a.D - R) >> 3;
+      const int unit = turn + (in == out ? 0 : rest);
+      for (int i = threadIdx.x; i < a.heads[w] * unit; i += kRopeThreads) {
+        const int h = i / unit, u = i - h * unit;
+        const T* x = in + h * a.in_sh[w];
+        T* y = out + h * a.out_sh[w];
+        if (u >= turn) {
+          const int d = R + (u - turn) * 8;
+          *(Pack8<T>*)(y + d) = *(const Pack8<T>*)(x + d);
+        } else if (kInter) {
+          const Pack8<T> v = *(const Pack8<T>*)(x + u * 8);
+          Pack8<T> o;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float y1, y2;
+            turn_pair(ld(v.v, 2 * j), ld(v.v, 2 * j + 1), cs[u * 4 + j], sn[u * 4 + j], y1, y2);
+            st(o.v, 2 * j, y1);
+            st(o.v, 2 * j + 1, y2);
+          }
+          *(Pack8<T>*)(y + u * 8) = o;
+        } else {
+          const Pack8<T> v1 = *(const Pack8<T>*)(x + u * 8), v2 = *(const Pack8<T>*)(x + a.pairs + u * 8);
+          Pack8<T> o1, o2;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float y1, y2;
+            turn_pair(ld(v1.v, j), ld(v2.v, j), cs[u * 8 + j], sn[u * 8 + j], y1, y2);
+            st(o1.v, j, y1);
+            st(o2.v, j, y2);
+          }
+          *(Pack8<T>*)(y + u * 8) = o1;
+          *(Pack8<T>*)(y + a.pairs + u * 8) = o2;
+        }
+      }
+    } else {
+      const int unit = a.pairs + (in == out ? 0 : a.D - R);
+      for (int i = threadIdx.x; i < a.heads[w] * unit; i += kRopeThreads) {
+        const int h = i / unit, u = i - h * unit;
+        const T* x = in + h * a.in_sh[w];
+        T* y = out + h * a.out_sh[w];
+        if (u >= a.pairs) {
+          y[R + u - a.pairs] = x[R + u - a.pairs];
+          continue;
+        }
+        const int d1 = kInter ? 2 * u : u, d2 = kInter ? 2 * u + 1 : a.pairs + u;
+        float y1, y2;
+        turn_pair(ld(x, d1), ld(x, d2), cs[u], sn[u], y1, y2);
+        st(y, d1, y1);
+        st(y, d2, y2);
+      }
+    }
+  }
+}
+
 int check_dtype(int dt, const char* who) {
   if (dt != GI_DTYPE_BF16 && dt != GI_DTYPE_FP16 && dt != GI_DTYPE_FP32)
     return fail(GI_ERR_UNSUPPORTED, std::string(who) + ": dtype must be bf16, fp16 or fp32");
@@ -164,6 +276,47 @@ int launch_rope(void* q, void* k, const void* cos_t, const void* sin_t, const in
   else GI_ROPE(float);
 #undef GI_ROPE
   return after_launch("rope launch");
+}
+
+int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, const int64_t* positions,
+                     const double* inv_freq, int dtype, int T, int Hq, int Hk, int D, int rotary_dim, int interleaved,
+                     float mscale, const int64_t* q_strides, const int64_t* qo_strides, const int64_t* k_strides,
+                     const int64_t* ko_strides, hipStream_t stream) {
+  int st = check_dtype(dtype, "rope_rows");
+  if (st != GI_OK) return st;
+  if (T < 0 || Hq < 0 || Hk < 0 || D <= 0 || rotary_dim <= 0 || rotary_dim > D || (rotary_dim & 1))
+    return fail(GI_ERR_INVALID_ARG, "rope_rows: T, Hq, Hk >= 0 and an even rotary_dim in [2, D] required");
+  if (rotary_dim > 2 * kRopeMaxPairs) return fail(GI_ERR_UNSUPPORTED, "rope_rows: rotary_dim at most 1024");
+  if (!k) Hk = 0;
+  if (T == 0 || Hq + Hk == 0) return GI_OK;
+  if ((Hq > 0 && (!q || !q_out)) || (Hk > 0 && !k_out) || !positions || !inv_freq)
+    return fail(GI_ERR_INVALID_ARG, "rope_rows: null pointer");
+  RopeArgs a{{q, k}, {q_out, k_out}, {q_strides[0], k_strides[0]}, {q_strides[1], k_strides[1]},
+             {qo_strides[0], ko_strides[0]}, {qo_strides[1], ko_strides[1]}, positions, inv_freq, mscale, {Hq, Hk}, D,
+             rotary_dim / 2};
+  const int size = dtype == GI_DTYPE_FP32 ? 4 : 2;
+  bool vec = D % 8 == 0 && rotary_dim % (interleaved ? 8 : 16) == 0;
+  for (int w = 0; w < 2; ++w) {
+    if (a.heads[w] == 0) continue;
+    vec = vec && ((uintptr_t)a.in[w] & 15) == 0 && ((uintptr_t)a.out[w] & 15) == 0;
+    for (const int64_t s : {a.in_st[w], a.in_sh[w], a.out_st[w], a.out_sh[w]}) vec = vec && s * size % 16 == 0;
+  }
+#define GI_ROPE_V(T_, I_)                                                                                      \
+  do {                                                                                                         \
+    if (vec) hipLaunchKernelGGL((rope_rows_kernel<T_, I_, true>), dim3(T), dim3(kRopeThreads), 0, stream, a);  \
+    else hipLaunchKernelGGL((rope_rows_kernel<T_, I_, false>), dim3(T), dim3(kRopeThreads), 0, stream, a);     \
+  } while (0)
+#define GI_ROPE_I(T_)                 \
+  do {                                \
+    if (interleaved) GI_ROPE_V(T_, true); \
+    else GI_ROPE_V(T_, false);        \
+  } while (0)
+  if (dtype == GI_DTYPE_BF16) GI_ROPE_I(uint16_t);
+  else if (dtype == GI_DTYPE_FP16) GI_ROPE_I(_Float16);
+  else GI_ROPE_I(float);
+#undef GI_ROPE_I
+#undef GI_ROPE_V
+  return after_launch("rope_rows launch");
 }
 
 }  // namespace gi

@@ -162,5 +162,26 @@ int launch_rmsnorm(const void* in, const void* weight, void* out, int dtype, int
 int launch_rope(void* q, void* k, const void* cos_t, const void* sin_t,
                 const int64_t* pos, int dtype, int B, int Hq, int Hk, int S, int D,
                 const int64_t* q_strides, const int64_t* k_strides, hipStream_t stream);
+// packed rows; strides are {row, head}
+int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, const int64_t* positions,
+                     const double* inv_freq, int dtype, int T, int Hq, int Hk, int D, int rotary_dim, int interleaved,
+                     float mscale, const int64_t* q_strides, const int64_t* qo_strides, const int64_t* k_strides,
+                     const int64_t* ko_strides, hipStream_t stream);
+
+// ---- 8-bit paged K/V cache (kv_cache.hip, kv_attention.hip) -------------------
+int launch_kv_slots(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* block_table, int max_pages,
+                    int64_t table_stride, const int32_t* free_pages, int n_free, const int32_t* free_used,
+                    int page_size, int64_t* slots, int64_t* positions, int n_tokens, int32_t* q_start,
+                    int32_t* seq_lens, int32_t* status, hipStream_t stream);
+int launch_kv_append(const void* k, const void* v, int dtype, const int64_t* k_strides, const int64_t* v_strides,
+                     const int64_t* slots, int T, int Hk, int D, int page_size, int64_t num_pages, void* k_cache,
+                     void* v_cache, float* k_scale, float* v_scale, hipStream_t stream);
+size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D);
+int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, const void* k_cache, const void* v_cache,
+                        const float* k_scale, const float* v_scale, const int32_t* block_table, int64_t table_stride,
+                        int max_pages, const int32_t* seq_lens, const int32_t* q_start, void* out,
+                        const int64_t* o_strides, int T, int B, int Hq, int Hk, int D, int page_size,
+                        int64_t num_pages, float scale, int window, void* workspace, size_t workspace_bytes,
+                        hipStream_t stream);
 
 }  // namespace gi

@@ -1,0 +1,592 @@
+// Attention of packed query rows over the 8-bit paged K/V cache (kv_cache.hip
+// has its layout): decode, verify and prompt chunks of grouped-query heads,
+// causal, with an optional sliding window.
+//
+//   s_j = scale * ks(page j) * (q . kcode_j),   p_j = exp(s_j - m) over the
+//   visible j, out = sum_j p_j vs(page j) vcode_j / sum_j p_j
+//
+// One pass over the cache with the running maximum and sum of a softmax.  The
+// G query heads of a kv head and the rows of a request are the columns of one
+// product: tile column r is row r / G, head r % G, so K and V are read once for
+// all of them.
+
+#include "../../include/gemmainfer_amd.h"
+#include "gi_common.h"
+#include "gi_internal.h"
+
+namespace gi {
+
+namespace {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kUnit = 64;      // cache rows a wave takes at a time
+constexpr int kMinChunk = 4;   // units: one a wave
+constexpr float kLog2e = 1.4426950408889634f;
+// Weights go to the matrix cores in fp16 as 2^(t - m + kBias), at most 2^(kBias
+// + kSlack): fp16 is normal down to 2^-14, so a weight 2^-21 of the largest
+// still has all 11 bits.
+constexpr float kBias = 7.f, kSlack = 8.f;
+
+struct AttnArgs {
+  const void* q;
+  int64_t q_st, q_sh;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const float* ks;
+  const float* vs;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  const int32_t* q_start;  // null: one row a request
+  void* out;
+  int64_t o_st, o_sh;
+  float* part;             // [items * Hk][RT][D] partial sums, then [items * Hk][RT] (maximum, sum)
+  int64_t num_pages;
+  float scale;             // with log2(e)
+  int T, B, Hk, G, cols, log_page, window, target, max_items;
+};
+
+// ---------------------------------------------------------------------------
+// the work list
+// ---------------------------------------------------------------------------
+// An item is (request, tile of RT columns, chunk of units); every workgroup
+// finds its own from the request lengths, on the device, so the launch needs no
+// host copy of them and can be replayed from a graph for other lengths.  The
+// chunk is the same for all requests: a long one is shared by as many
+// workgroups as a batch of short ones.
+struct Item {
+  int b, tile, tiles, chunk_no, chunk, q0, rows, len, first_item;
+  bool over;  // longer than the table: its pages cannot all be there
+};
+
+struct Load {
+  int q0, rows, len, tiles, units;
+  bool over;
+};
+
+template <int RT>
+__device__ __forceinline__ Load load_of(const AttnArgs& a, int b) {
+  Load r{0, 0, 0, 0, 0, false};
+  if (b >= a.B) return r;
+  int q0 = b, q1 = b + 1;
+  if (a.q_start) {
+    q0 = min(max(a.q_start[b], 0), a.T);
+    q1 = min(max(a.q_start[b + 1], q0), a.T);
+  }
+  const int64_t cap = (int64_t)a.cols << a.log_page;
+  const int64_t len = max(a.lens[b], 0);
+  r.q0 = q0;
+  r.rows = q1 - q0;
+  r.over = len > cap;
+  r.len = (int)min(len, cap);
+  r.tiles = (int)(((int64_t)r.rows * a.G + RT - 1) / RT);
+  int units = (r.len + kUnit - 1) / kUnit;
+  if (a.window > 0) units = (int)min((int64_t)units, ((int64_t)a.window + RT) / kUnit + 2);
+  r.units = units;
+  return r;
+}
+
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int u = __shfl_up(v, off, kWave);
+    if (lane >= off) v += u;
+  }
+  return v;
+}
+
+// Item `want` of the list (by_tile: the first item of tile `want`); false past its end.
+template <int RT>
+__device__ __forceinline__ bool find_item(const AttnArgs& a, int want, bool by_tile, Item& it) {
+  const int lane = threadIdx.x & 63;
+  const Load head = load_of<RT>(a, lane);
+  long long total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
+    total += (long long)l.tiles * l.units;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, kWave);
+  const int chunk = (int)max((total + a.target - 1) / a.target, (long long)kMinChunk);
+  int items = 0, tiles = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
+    const int chunks = max((l.units + chunk - 1) / chunk, 1);
+    const int n = l.tiles * chunks;
+    const int item_end = items + wave_scan(n), tile_end = tiles + wave_scan(l.tiles);
+    const int end = by_tile ? tile_end : item_end, first = end - (by_tile ? l.tiles : n);
+    const unsigned long long hit = __ballot(want >= first && want < end);
+    if (hit) {
+      const int src = __ffsll(hit) - 1;
+      const int in = want - __shfl(first, src, kWave);
+      const int per = __shfl(chunks, src, kWave);
+      const int first_item = __shfl(item_end - n, src, kWave);
+      it.b = b0 + src;
+      it.tile = by_tile ? in : in / per;
+      it.chunk_no = by_tile ? 0 : in - it.tile * per;
+      it.tiles = __shfl(l.tiles, src, kWave);
+      it.chunk = chunk;
+      it.q0 = __shfl(l.q0, src, kWave);
+      it.rows = __shfl(l.rows, src, kWave);
+      it.len = __shfl(l.len, src, kWave);
+      it.over = __shfl((int)l.over, src, kWave);
+      it.first_item = first_item + it.tile * per;
+      // the last tiles of a prompt see the most: they go first
+      it.tile = it.tiles - 1 - it.tile;
+      return true;
+    }
+    items = __shfl(item_end, kWave - 1, kWave);
+    tiles = __shfl(tile_end, kWave - 1, kWave);
+  }
+  return false;
+}
+
+// What a tile's columns see: units [lo, hi), and how many chunks they are cut into.
+struct Span {
+  int lo, hi, chunks;
+  int pos_min, pos_max;  // positions of its first and last row
+};
+
+template <int RT>
+__device__ __forceinline__ Span span_of(const AttnArgs& a, const Item& it) {
+  Span s;
+  const int64_t r0 = (int64_t)it.tile * RT, r1 = min(r0 + RT, (int64_t)it.rows * a.G) - 1;
+  s.pos_min = it.len - it.rows + (int)(r0 / a.G);
+  s.pos_max = it.len - it.rows + (int)(r1 / a.G);
+  s.lo = 0;
+  if (a.window > 0) s.lo = max(s.pos_min - a.window + 1, 0) / kUnit;
+  s.hi = s.pos_max < 0 ? 0 : s.pos_max / kUnit + 1;
+  s.chunks = max((s.hi - s.lo + it.chunk - 1) / it.chunk, 1);
+  return s;
+}
+
+// ---------------------------------------------------------------------------
+// types of the first product (the second one is fp16 for both)
+// ---------------------------------------------------------------------------
+template <bool F16>
+struct Qk;
+template <>
+struct Qk<false> {
+  typedef bf16x8_t frag;
+  static __device__ __forceinline__ frag codes(uint32_t lo, uint32_t hi) {
+    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false);
+    const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+    const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false);
+    const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+    return frag{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+  }
+  static __device__ __forceinline__ f32x4_t mfma(frag a, frag b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint16_t out(float f) { return f32_to_bf16(f); }
+};
+
+__device__ __forceinline__ f16x8_t codes_f16(uint32_t lo, uint32_t hi) {
+  const f16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+  const f16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+  const f16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+  const f16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  return f16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ f32x4_t mfma_f16(f16x8_t a, f16x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+template <>
+struct Qk<true> {
+  typedef f16x8_t frag;
+  static __device__ __forceinline__ frag codes(uint32_t lo, uint32_t hi) { return codes_f16(lo, hi); }
+  static __device__ __forceinline__ f32x4_t mfma(frag a, frag b, f32x4_t c) { return mfma_f16(a, b, c); }
+  static __device__ __forceinline__ uint16_t out(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+};
+
+// ---------------------------------------------------------------------------
+// the kernel
+// ---------------------------------------------------------------------------
+// The four waves of a workgroup take turns at units of 64 cache rows; each has
+// its own running softmax over 16 * CT columns, joined at the end through LDS.
+// No barrier and no LDS in the loop: lane (i = lane % 16, g = lane / 16) reads
+// from the cache just what its place in the MFMA operands needs.
+//   S^T = K Q^T, 16x16x32: operand A's row i of product j is cache row 16 (i / 4) +
+//     4 j + i % 4 of the unit, so that the four results of lane (i, g) are rows
+//     16 g + 4 j ... + 3 of column i: after j = 0..3 a lane holds the 16
+//     rows of ITS group g, one page's rows, in order.
+//   O^T = V^T P^T: operand B wants 8 rows of column i from lane (i, g): those
+//     are its own scores.  Operand A is 16 rows of dimension 16 dt + i, one
+//     16-byte load of the transposed V.
+// So neither the scores nor V cross lanes, and a lane needs one K and one V
+// scale per unit.  A column's maximum is the only exchange (two lane swaps).
+//
+// V's scale joins the exponent: t = s + log2(vs), weights 2^(t - m), m over t.
+// The sum of softmax weights is then sum 2^(t - m) / vs.  With it the weights
+// of V's codes never exceed 2^(kBias + kSlack) whatever the scales are, and the
+// maximum is over what each row can contribute.
+template <int D, int CT, bool F16>
+__global__ __launch_bounds__(kThreads, 1) void kv_attention_kernel(AttnArgs a) {
+  constexpr int RT = 16 * CT;
+  constexpr int KS = D / 64;   // 16-byte K loads of a lane per row
+  constexpr int DT = D / 16;   // dimension tiles of the output
+  constexpr bool kQLds = CT * D > 512;
+  typedef typename Qk<F16>::frag frag;
+  __shared__ float red[RT][D + 4];
+  __shared__ float red_m[kWaves][RT], red_l[kWaves][RT];
+  __shared__ uint4 q_lds[kQLds ? CT * 2 * KS * kWave : 1];
+
+  const int hk = blockIdx.x % a.Hk;
+  Item it;
+  if (!find_item<RT>(a, blockIdx.x / a.Hk, false, it)) return;
+  const Span sp = span_of<RT>(a, it);
+  if (it.chunk_no >= sp.chunks) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i16 = lane & 15, g = lane >> 4;
+  const int page_mask = (1 << a.log_page) - 1;
+  const int r0 = it.tile * RT;
+  const int n_cols = (int)min((int64_t)RT, (int64_t)it.rows * a.G - r0);
+
+  // ---- Q as operand B: column i, dimensions 64 s + 16 g + 8 h ... of step 2 s + h
+  frag qf[kQLds ? 1 : CT][kQLds ? 1 : 2 * KS];
+  int hi_pos[CT];  // the column's position: it sees rows up to it
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = ct * 16 + i16, r = r0 + min(c, n_cols - 1);
+    const int row = r / a.G, head = hk * a.G + (r - row * a.G);
+    hi_pos[ct] = it.len - it.rows + row;
+    const uint16_t* src = (const uint16_t*)a.q + (it.q0 + row) * a.q_st + head * a.q_sh;
+#pragma unroll
+    for (int s = 0; s < 2 * KS; ++s) {
+      if (kQLds && (ct * 2 * KS + s) % kWaves != wave) continue;
+      const uint4 w = *(const uint4*)(src + (s >> 1) * 64 + g * 16 + (s & 1) * 8);
+      if (kQLds) q_lds[(ct * 2 * KS + s) * kWave + lane] = w;
+      else qf[kQLds ? 0 : ct][kQLds ? 0 : s] = __builtin_bit_cast(frag, w);
+    }
+  }
+  if (kQLds) __syncthreads();
+
+  f32x4_t acc[CT][DT];
+  float m[CT], mref[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = -INFINITY;
+    mref[ct] = 0.f;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[ct][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int32_t* table = a.table + it.b * a.table_stride;
+  auto page_of = [&](int tok) -> int64_t {
+    const int col = tok >> a.log_page;
+    return col < a.cols ? (int64_t)table[col] : (int64_t)-1;
+  };
+  const int u_end = min(sp.lo + (it.chunk_no + 1) * it.chunk, sp.hi);
+  const int u_first = sp.lo + it.chunk_no * it.chunk + wave;
+  const int grp_k = 16 * (i16 >> 2);
+  for (int u = u_first; u < u_end; u += kWaves) {
+    const int tok = u * kUnit;
+    int64_t kp = page_of(tok + grp_k), vp = page_of(tok + 16 * g);
+    // a page that is not there: nothing is read from where it points, and its
+    // rows, if they are seen at all, have no scale
+    if (kp < 0 || kp >= a.num_pages) kp = 0;
+    const bool bad = vp < 0 || vp >= a.num_pages || it.over;
+    if (vp < 0 || vp >= a.num_pages) vp = 0;
+    const uint8_t* kb = a.kc + (((kp * a.Hk + hk) << a.log_page) + ((tok + grp_k) & page_mask) + (i16 & 3)) * D + 16 * g;
+    const uint8_t* vb = a.vc + (((vp * a.Hk + hk) * D + i16) << a.log_page) + ((tok + 16 * g) & page_mask);
+    float ks = a.ks[vp * a.Hk + hk], vs = a.vs[vp * a.Hk + hk];
+    if (bad) ks = vs = __uint_as_float(0x7fc00000u);
+
+    // ---- scores
+    f32x4_t s[CT][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) s[ct][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        const uint4 w = *(const uint4*)(kb + j * 4 * D + st * 64);
+        const frag k0 = Qk<F16>::codes(w.x, w.y), k1 = Qk<F16>::codes(w.z, w.w);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const frag q0 = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * st) * kWave + lane])
+                                : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * st];
+          const frag q1 = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * st + 1) * kWave + lane])
+                                : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * st + 1];
+          s[ct][j] = Qk<F16>::mfma(k0, q0, s[ct][j]);
+          s[ct][j] = Qk<F16>::mfma(k1, q1, s[ct][j]);
+        }
+      }
+    }
+
+    // ---- weights
+    const float cs = ks * a.scale, cv = __log2f(vs), inv_vs = 1.f / vs;
+    const bool edge = tok + kUnit - 1 > sp.pos_min || (a.window > 0 && tok <= sp.pos_max - a.window);
+    f16x8_t p[CT][2];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float t = fmaf(s[ct][j][r], cs, cv);
+          if (edge) {
+            const int x = tok + 16 * g + 4 * j + r;
+            const bool seen = x <= hi_pos[ct] && (a.window <= 0 || x > hi_pos[ct] - a.window);
+            t = seen ? t : -INFINITY;
+          }
+          s[ct][j][r] = t;
+          top = fmaxf(top, t);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      if (__any(top > m[ct] + kSlack)) {
+        const float now = fmaxf(m[ct], top);
+        const float next = now == -INFINITY ? 0.f : now;
+        const float f = m[ct] == -INFINITY ? 0.f : exp2f(mref[ct] - next);  // -inf: nothing was added yet
+        m[ct] = now;
+        mref[ct] = next;
+        l[ct] *= f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[ct][dt] *= f;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float w = exp2f(s[ct][j][r] - mref[ct] + kBias);
+          sum += w;
+          p[ct][j >> 1][(j & 1) * 4 + r] = (_Float16)w;
+        }
+      }
+      // rows that are not seen weigh nothing, whatever their page's scale is
+      l[ct] += sum == 0.f ? 0.f : sum * inv_vs;
+    }
+
+    // ---- O^T += V^T P^T
+    const int last = min(sp.pos_max - (tok + 16 * g), 15), firstx = a.window > 0 ? sp.pos_min - a.window + 1 - (tok + 16 * g) : 0;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      uint4 w = *(const uint4*)(vb + ((dt * 16) << a.log_page));
+      if (edge) {  // rows that no column sees may hold anything
+        uint32_t o[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if (x > last || x < firstx) o[x >> 2] &= ~(0xffu << (8 * (x & 3)));
+        w = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      const f16x8_t v0 = codes_f16(w.x, w.y), v1 = codes_f16(w.z, w.w);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        acc[ct][dt] = mfma_f16(v0, p[ct][0], acc[ct][dt]);
+        acc[ct][dt] = mfma_f16(v1, p[ct][1], acc[ct][dt]);
+      }
+    }
+  }
+
+  // ---- join the waves
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    l[ct] += __shfl_xor(l[ct], 16, kWave);
+    l[ct] += __shfl_xor(l[ct], 32, kWave);
+    if (g == 0) {
+      red_m[wave][ct * 16 + i16] = m[ct] == -INFINITY ? -INFINITY : mref[ct];
+      red_l[wave][ct * 16 + i16] = l[ct];
+    }
+  }
+  __syncthreads();
+  float f[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red_m[w][ct * 16 + i16]);
+    f[ct] = m[ct] == -INFINITY ? 0.f : exp2f(mref[ct] - top);
+  }
+  for (int w = 0; w < kWaves; ++w) {
+    if (w == wave) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x4_t* dst = (f32x4_t*)&red[ct * 16 + i16][dt * 16 + 4 * g];
+          const f32x4_t v = acc[ct][dt] * f[ct];
+          *dst = w == 0 ? v : *dst + v;
+        }
+    }
+    __syncthreads();
+  }
+  for (int e = threadIdx.x; e < n_cols * (D / 8); e += kThreads) {
+    const int c = e / (D / 8), d = (e - c * (D / 8)) * 8;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red_m[w][c]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      if (red_m[w][c] != -INFINITY) sum += red_l[w][c] * exp2f(red_m[w][c] - top);
+    if (sp.chunks == 1) {
+      const int r = r0 + c, row = r / a.G, head = hk * a.G + (r - row * a.G);
+      uint16_t o[8];
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) o[x] = Qk<F16>::out(red[c][d + x] * inv);
+      *(uint4*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
+          make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
+    } else {
+      float* dst = a.part + ((size_t)blockIdx.x * RT + c) * D + d;
+      *(float4*)dst = make_float4(red[c][d], red[c][d + 1], red[c][d + 2], red[c][d + 3]);
+      *(float4*)(dst + 4) = make_float4(red[c][d + 4], red[c][d + 5], red[c][d + 6], red[c][d + 7]);
+      if (d == 0) {
+        float* ml = a.part + (size_t)a.max_items * a.Hk * RT * D + ((size_t)blockIdx.x * RT + c) * 2;
+        ml[0] = top;
+        ml[1] = sum;
+      }
+    }
+  }
+}
+
+// Joins the chunks of tiles that were cut: out = sum_c 2^(m_c - m) O_c / sum_c
+// 2^(m_c - m) l_c, in the order of the chunks.  A thread takes four dimensions
+// of a column.
+template <int D, int CT, bool F16>
+__global__ __launch_bounds__(kThreads) void kv_attention_join_kernel(AttnArgs a) {
+  constexpr int RT = 16 * CT;
+  const int hk = blockIdx.x % a.Hk;
+  Item it;
+  if (!find_item<RT>(a, blockIdx.x / a.Hk, true, it)) return;
+  const Span sp = span_of<RT>(a, it);
+  if (sp.chunks == 1 || it.first_item + sp.chunks > a.max_items) return;
+  const int e = blockIdx.y * kThreads + threadIdx.x;
+  const int c = e / (D / 4), d = (e - c * (D / 4)) * 4;
+  const int r = it.tile * RT + c;
+  if (c >= RT || r >= it.rows * a.G) return;
+  const float* ml = a.part + (size_t)a.max_items * a.Hk * RT * D;
+  float top = -INFINITY;
+  for (int n = 0; n < sp.chunks; ++n) top = fmaxf(top, ml[(((size_t)(it.first_item + n) * a.Hk + hk) * RT + c) * 2]);
+  float sum = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < sp.chunks; ++n) {
+    const size_t at = ((size_t)(it.first_item + n) * a.Hk + hk) * RT + c;
+    const float mm = ml[at * 2];
+    const float f = mm == -INFINITY ? 0.f : exp2f(mm - top);
+    sum += f * ml[at * 2 + 1];
+    o += f * *(const f32x4_t*)(a.part + at * D + d);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int row = r / a.G, head = hk * a.G + (r - row * a.G);
+  uint16_t b[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) b[x] = Qk<F16>::out(o[x] * inv);
+  *(uint2*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
+      make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+}
+
+int after_launch(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? GI_OK : hip_fail(e, what);
+}
+
+int col_tiles(int T, int B, int G, int D) {
+  const int64_t rows = ((int64_t)T * G + B - 1) / B;
+  if (rows <= 16) return 1;
+  if (rows <= 32 || D > 256) return 2;
+  return 4;
+}
+
+struct Grid {
+  int ct, target, max_items, max_tiles;
+};
+
+Grid grid_of(int T, int B, int Hq, int Hk, int D) {
+  const int G = Hq / Hk;
+  Grid r;
+  r.ct = col_tiles(T, B, G, D);
+  const int RT = 16 * r.ct;
+  const int64_t cols = (int64_t)T * G;
+  r.max_tiles = (int)(cols < cols / RT + B ? cols : cols / RT + B);
+  r.target = (2 * 256 + Hk - 1) / Hk;
+  r.max_items = r.target + r.max_tiles;
+  return r;
+}
+
+size_t part_bytes(const Grid& gr, int Hk, int D) {
+  return (size_t)gr.max_items * Hk * gr.ct * 16 * (D + 2) * sizeof(float);
+}
+
+bool width_ok(int D) { return D == 64 || D == 128 || D == 256 || D == 512; }
+
+template <int D, int CT, bool F16>
+void launch(const AttnArgs& a, const Grid& gr, hipStream_t stream) {
+  hipLaunchKernelGGL((kv_attention_kernel<D, CT, F16>), dim3(gr.max_items * a.Hk), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((kv_attention_join_kernel<D, CT, F16>), dim3(gr.max_tiles * a.Hk, (16 * CT * D / 4 + kThreads - 1) / kThreads),
+                     dim3(kThreads), 0, stream, a);
+}
+
+template <int D, bool F16>
+void launch_ct(const AttnArgs& a, const Grid& gr, hipStream_t stream) {
+  if (gr.ct == 1) launch<D, 1, F16>(a, gr, stream);
+  else if (gr.ct == 2) launch<D, 2, F16>(a, gr, stream);
+  else if constexpr (D <= 256) launch<D, 4, F16>(a, gr, stream);
+}
+
+template <bool F16>
+void launch_d(const AttnArgs& a, const Grid& gr, int D, hipStream_t stream) {
+  if (D == 64) launch_ct<64, F16>(a, gr, stream);
+  else if (D == 128) launch_ct<128, F16>(a, gr, stream);
+  else if (D == 256) launch_ct<256, F16>(a, gr, stream);
+  else launch_ct<512, F16>(a, gr, stream);
+}
+
+}  // namespace
+
+size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D) {
+  if (T <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || !width_ok(D)) return 0;
+  return part_bytes(grid_of(T, B, Hq, Hk, D), Hk, D);
+}
+
+int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, const void* k_cache, const void* v_cache,
+                        const float* k_scale, const float* v_scale, const int32_t* block_table, int64_t table_stride,
+                        int max_pages, const int32_t* seq_lens, const int32_t* q_start, void* out,
+                        const int64_t* o_strides, int T, int B, int Hq, int Hk, int D, int page_size,
+                        int64_t num_pages, float scale, int window, void* workspace, size_t workspace_bytes,
+                        hipStream_t stream) {
+  if (dtype != GI_DTYPE_BF16 && dtype != GI_DTYPE_FP16)
+    return fail(GI_ERR_UNSUPPORTED, "kv_attention: query rows must be bf16 or fp16");
+  if (T < 0 || B < 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || max_pages < 0 || table_stride < max_pages || num_pages < 0)
+    return fail(GI_ERR_INVALID_ARG, "kv_attention: bad shape (Hq must be a multiple of Hk, table_stride >= max_pages)");
+  if (!width_ok(D)) return fail(GI_ERR_UNSUPPORTED, "kv_attention: head widths 64, 128, 256 and 512");
+  int lp = -1;
+  for (int l = 4; l <= 8; ++l)
+    if (page_size == 1 << l) lp = l;
+  if (lp < 0) return fail(GI_ERR_INVALID_ARG, "kv_attention: page_size must be 16, 32, 64, 128 or 256");
+  if (!q_start && T != B) return fail(GI_ERR_INVALID_ARG, "kv_attention: without q_start there is one row a request");
+  if (!(scale == scale)) return fail(GI_ERR_INVALID_ARG, "kv_attention: scale is NaN");
+  if (window < 0) return fail(GI_ERR_INVALID_ARG, "kv_attention: window must be >= 0 (0: none)");
+  if ((int64_t)T * (Hq / Hk) > 0x3fffffff || (int64_t)max_pages * page_size > 0x3fffffff)
+    return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows, or a table of more than 2^30 tokens");
+  if (T == 0 || B == 0) return GI_OK;
+  if (num_pages == 0) return fail(GI_ERR_INVALID_ARG, "kv_attention: the cache has no pages");
+  if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !seq_lens || !out || (max_pages > 0 && !block_table))
+    return fail(GI_ERR_INVALID_ARG, "kv_attention: null pointer");
+  for (const void* p : {q, k_cache, v_cache, (const void*)out})
+    if ((uintptr_t)p & 15) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
+  for (const int64_t s : {q_strides[0], q_strides[1], o_strides[0], o_strides[1]})
+    if (s % 8) return fail(GI_ERR_INVALID_ARG, "kv_attention: row and head strides must be multiples of 8 elements");
+  const Grid gr = grid_of(T, B, Hq, Hk, D);
+  if ((int64_t)gr.max_items * Hk > 0x7fffffff) return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows");
+  if (!workspace || workspace_bytes < part_bytes(gr, Hk, D))
+    return fail(GI_ERR_WORKSPACE, "kv_attention: workspace missing or too small");
+  AttnArgs a{q, q_strides[0], q_strides[1], (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale,
+             block_table, table_stride, seq_lens, q_start, out, o_strides[0], o_strides[1], (float*)workspace,
+             num_pages, scale * kLog2e, T, B, Hk, Hq / Hk, max_pages, lp, window, gr.target, gr.max_items};
+  if (dtype == GI_DTYPE_FP16) launch_d<true>(a, gr, D, stream);
+  else launch_d<false>(a, gr, D, stream);
+  return after_launch("kv_attention launch");
+}
+
+}  // namespace gi

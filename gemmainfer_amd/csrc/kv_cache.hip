@@ -1,0 +1,446 @@
+// The 8-bit paged K/V cache: where the rows of a step go (kv_slots) and how
+// they are stored (kv_append).  kv_attention.hip reads it.
+//
+// Layout.  A page holds P rows (tokens) of every kv head as OCP e4m3 codes,
+//   k_cache [pages, Hk, P, D]   a row's D codes together
+//   v_cache [pages, Hk, D, P]   a dimension's P codes together
+// and one fp32 scale per (page, head) for K and one for V: value = code *
+// scale.  V is held transposed because the matrix cores contract P.V over
+// rows: a lane then reads 16 rows of its dimension with one 16-byte load, where
+// [P, D] would need a transposition in registers or LDS for every page on every
+// decode step.  The price is paid once per row, at append: a lone row's V codes
+// are single bytes P apart.
+//
+// Scales are powers of two, the smallest that brings the page's largest value
+// under 448 (the largest e4m3).  With those, x / scale is exact, a stored value
+// code * scale is exact in bf16 and fp32, and when a larger row arrives the
+// page's codes move to the larger scale by a change of exponent (rounded only
+// where they fall under e4m3's smallest normal number).
+
+#include "../../include/gemmainfer_amd.h"
+#include "gi_common.h"
+#include "gi_internal.h"
+
+namespace gi {
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// kv_slots
+// ---------------------------------------------------------------------------
+// One launch, no exchange between workgroups: each scans the B request lengths
+// into its own LDS (12 bytes of global reads a request) and then places its
+// 256 tokens.  A fresh page j of a request starts at position j*P >= ctx, which
+// is one of the call's own tokens: that token's thread writes the table entry,
+// so table entries are never read and written in one call.  Bound by latency
+// (lengths -> scan -> table entry -> slot).
+constexpr int kSlotThreads = 256;
+constexpr int kMaxRequests = 8192;  // two ints a request in LDS: 64 KB
+
+struct SlotArgs {
+  const int32_t* ctx;
+  const int32_t* add;
+  int32_t* table;
+  const int32_t* free_pages;
+  const int32_t* used;
+  int64_t* slots;
+  int64_t* positions;
+  int32_t* q_start;
+  int32_t* seq_lens;
+  int32_t* status;
+  int64_t table_stride;
+  int B, cols, n_free, log_page, n;
+};
+
+// Inclusive scan over the workgroup; `total` gets the sum.  Two barriers.
+template <typename I>
+__device__ __forceinline__ I block_scan(I v, I* part, I& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const I u = __shfl_up(v, off, kWave);
+    if (lane >= off) v += u;
+  }
+  __syncthreads();  // the previous scan's readers are done with `part`
+  if (lane == 63) part[wave] = v;
+  __syncthreads();
+  I before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSlotThreads / kWave; ++w) {
+    if (w < wave) before += part[w];
+    total += part[w];
+  }
+  return v + before;
+}
+
+__global__ __launch_bounds__(kSlotThreads) void kv_slots_kernel(SlotArgs a) {
+  extern __shared__ int lds[];
+  int* start = lds;         // [B] first row of each request, at most n
+  int* fresh = lds + a.B;   // [B] fresh pages of the requests before it
+  __shared__ long long part64[kSlotThreads / kWave];
+  __shared__ int part32[kSlotThreads / kWave];
+  const int tid = threadIdx.x;
+  const int up = (1 << a.log_page) - 1;
+  long long rows = 0, lack = 0;  // rows asked for so far; pages behind the table's last column
+  int pages = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kSlotThreads) {
+    const int b = b0 + tid;
+    const bool on = b < a.B;
+    const long long ctx = on ? max(a.ctx[b], 0) : 0;
+    const long long add = on ? max(a.add[b], 0) : 0;
+    long long sum;
+    const long long end = rows + block_scan<long long>(add, part64, sum);
+    rows += sum;
+    const long long first = min(end - add, (long long)a.n);
+    const long long len = ctx + min(add, (long long)a.n - first);
+    const long long have = (ctx + up) >> a.log_page, want = (len + up) >> a.log_page;
+    const int count = (int)(min(want, (long long)a.cols) - min(have, (long long)a.cols));
+    lack += want - have - count;
+    int psum;
+    const int pend = pages + block_scan<int>(count, part32, psum);
+    pages += psum;
+    if (on) {
+      start[b] = (int)first;
+      fresh[b] = pend - count;
+      if (blockIdx.x == 0) {
+        a.q_start[b] = (int)first;
+        a.seq_lens[b] = (int)min(len, 0x7fffffffLL);
+      }
+    }
+  }
+  const int live = (int)min(rows, (long long)a.n);
+  const int used = max(a.used[0], 0);
+  if (blockIdx.x == 0) {
+    long long all;
+    block_scan<long long>(lack, part64, all);
+    if (tid == 0) {
+      const int got = min(pages, max(a.n_free - used, 0));
+      a.q_start[a.B] = live;
+      a.status[0] = used + got;
+      a.status[1] = (int)min(all + pages - got, 0x7fffffffLL);
+      a.status[2] = (int)min(rows - live, 0x7fffffffLL);
+    }
+  }
+  __syncthreads();
+  const int t = blockIdx.x * kSlotThreads + tid;
+  if (t >= a.n) return;
+  long long slot = -1, pos = 0;
+  if (t < live) {
+    int lo = 0, hi = a.B - 1;  // the last request whose first row is at most t
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (start[mid] <= t) lo = mid;
+      else hi = mid - 1;
+    }
+    const long long ctx = max(a.ctx[lo], 0);
+    pos = ctx + (t - start[lo]);
+    const long long j = pos >> a.log_page, have = (ctx + up) >> a.log_page;
+    if (j < a.cols) {
+      int32_t* entry = a.table + lo * a.table_stride + j;
+      long long page;
+      if (j < have) {
+        page = *entry;
+      } else {
+        const long long at = (long long)used + fresh[lo] + (j - have);
+        page = at < a.n_free ? a.free_pages[at] : -1;
+        if ((pos & up) == 0) *entry = (int)page;
+      }
+      if (page >= 0) slot = (page << a.log_page) + (pos & up);
+    }
+  }
+  a.slots[t] = slot;
+  a.positions[t] = pos;
+}
+
+// ---------------------------------------------------------------------------
+// kv_append
+// ---------------------------------------------------------------------------
+constexpr int kAppThreads = 256;
+constexpr int kMaxPage = 256;
+
+struct AppendArgs {
+  const void* x[2];        // K rows, V rows
+  int64_t st[2], sh[2];    // row and head strides, elements
+  const int64_t* slots;
+  uint8_t* cache[2];
+  float* scale[2];
+  int64_t num_pages;
+  int T, Hk, D, log_page, per_wg;
+};
+
+template <typename T>
+struct Vec8;  // eight consecutive elements as floats
+template <>
+struct Vec8<uint16_t> {
+  static __device__ __forceinline__ void load(const uint16_t* p, float* f) {
+    const uint4 d = *(const uint4*)p;
+    const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = bf16lo(w[i]);
+      f[2 * i + 1] = bf16hi(w[i]);
+    }
+  }
+  static __device__ __forceinline__ float one(const uint16_t* p) { return bf16_to_f32(*p); }
+};
+template <>
+struct Vec8<_Float16> {
+  static __device__ __forceinline__ void load(const _Float16* p, float* f) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    const h8 d = *(const h8*)p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)d[i];
+  }
+  static __device__ __forceinline__ float one(const _Float16* p) { return (float)*p; }
+};
+template <>
+struct Vec8<float> {
+  static __device__ __forceinline__ void load(const float* p, float* f) {
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  }
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+};
+
+template <typename T, bool kVec>
+__device__ __forceinline__ void load8(const T* p, float* f) {
+  if (kVec) {
+    Vec8<T>::load(p, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = Vec8<T>::one(p + i);
+  }
+}
+
+// e4m3 codes of four values (round to nearest even; |f| <= 448).
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+// The codes of `w` for a scale 1/ratio times the old one.
+__device__ __forceinline__ uint32_t rescale_e4m3(uint32_t w, float ratio) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return pack_e4m3(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio);
+}
+
+// The smallest power of two s in [2^-40, 2^40] with amax <= 448 s (448 = 1.75 *
+// 2^8), from amax's bits; NaN where there is none (amax infinite, NaN or larger).
+__device__ __forceinline__ float page_scale(uint32_t amax_bits) {
+  int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  if (e > 40) return __uint_as_float(0x7fc00000u);
+  e = max(e, -40);
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// One workgroup a (run of rows, head, K or V); a run is the rows of the call
+// that follow each other on one page, and its first row's workgroup does it
+// all: which row lands on each of the page's P places (the last one wins where
+// a slot is named twice), the largest value of those rows, the page's scale,
+// then the codes.  Everything of a page in one workgroup needs no atomics on
+// scales and no second launch.  Reads the rows twice; the second time they
+// come from the caches.  per_wg rows are looked at by one workgroup.
+template <typename T, bool kVec>
+__global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
+  __shared__ int last[kMaxPage];
+  __shared__ uint32_t wave_max[kAppThreads / kWave];
+  __shared__ int run_end;
+  const int tid = threadIdx.x, head = blockIdx.y, kv = blockIdx.z;
+  const int P = 1 << a.log_page, D = a.D;
+  const T* x = (const T*)a.x[kv] + head * a.sh[kv];
+  const int64_t st = a.st[kv];
+  const int t_end = min((int)(blockIdx.x + 1) * a.per_wg, a.T);
+  for (int t0 = blockIdx.x * a.per_wg; t0 < t_end; ++t0) {
+    const int64_t slot = a.slots[t0];
+    const int64_t page = slot >> a.log_page;
+    if (slot < 0 || page >= a.num_pages) continue;
+    if (t0 > 0 && a.slots[t0 - 1] >> a.log_page == page) continue;
+    __syncthreads();  // the previous run's readers of LDS are done
+    for (int p = tid; p < P; p += kAppThreads) last[p] = -1;
+    // ---- the run's rows
+    for (int base = t0;; base += kAppThreads) {
+      if (tid == 0) run_end = base + kAppThreads;
+      __syncthreads();
+      const int t = base + tid;
+      const int64_t s = t < a.T ? a.slots[t] : -1;
+      const bool same = s >= 0 && s >> a.log_page == page;
+      if (!same) atomicMin(&run_end, t);
+      __syncthreads();
+      const int end = run_end;
+      if (t < end) atomicMax(&last[s & (P - 1)], t);
+      __syncthreads();
+      if (end < base + kAppThreads) break;
+    }
+    // ---- their largest value
+    const int per_row = D >> 3;  // threads of 8 elements
+    uint32_t m = 0;
+    for (int i = tid; i < P * per_row; i += kAppThreads) {
+      const int p = i / per_row, c = (i - p * per_row) << 3;
+      const int t = last[p];
+      if (t < 0) continue;
+      float f[8];
+      load8<T, kVec>(x + t * st + c, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, kWave));
+    if ((tid & 63) == 0) wave_max[tid >> 6] = m;
+    float* scale = a.scale[kv] + page * a.Hk + head;
+    const float old = *scale;
+    __syncthreads();
+    m = max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]));
+    const float need = page_scale(m);
+    const bool restart = last[0] >= 0;
+    float now = need;
+    if (!restart && !(old < need)) now = need == need ? old : need;  // old >= need, or one of them NaN
+    if (tid == 0) *scale = now;
+    const bool valid = now == now;
+    const float inv = valid ? 1.f / now : 0.f;                       // a page without a scale holds zeros
+    const bool move = !restart && valid && now > old;
+    const float ratio = move ? old * inv : 1.f;
+    uint8_t* codes = a.cache[kv] + (page * a.Hk + head) * ((int64_t)D << a.log_page);
+    if (kv == 0) {
+      for (int i = tid; i < P * per_row; i += kAppThreads) {
+        const int p = i / per_row, c = (i - p * per_row) << 3;
+        const int t = last[p];
+        uint2* dst = (uint2*)(codes + (int64_t)p * D + c);
+        if (t >= 0) {
+          float f[8];
+          load8<T, kVec>(x + t * st + c, f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = valid ? f[j] * inv : 0.f;
+          *dst = make_uint2(pack_e4m3(f[0], f[1], f[2], f[3]), pack_e4m3(f[4], f[5], f[6], f[7]));
+        } else if (move) {
+          const uint2 w = *dst;
+          *dst = make_uint2(rescale_e4m3(w.x, ratio), rescale_e4m3(w.y, ratio));
+        }
+      }
+    } else {
+      // a thread takes one dimension of 16 places: its codes are 16 adjacent bytes
+      for (int i = tid; i < D * (P >> 4); i += kAppThreads) {
+        const int g = i / D, d = i - g * D;
+        uint8_t* dst = codes + ((int64_t)d << a.log_page) + g * 16;
+        int n_new = 0;
+#pragma unroll
+        for (int p = 0; p < 16; ++p) n_new += last[g * 16 + p] >= 0;
+        if (n_new == 0 && !move) continue;
+        if (n_new == 16 || move) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (n_new < 16) {
+            w = *(const uint4*)dst;
+            w = make_uint4(rescale_e4m3(w.x, ratio), rescale_e4m3(w.y, ratio), rescale_e4m3(w.z, ratio),
+                           rescale_e4m3(w.w, ratio));
+          }
+          uint32_t o[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int p = 0; p < 16; ++p) {
+            const int t = last[g * 16 + p];
+            if (t < 0) continue;
+            const float f = valid ? Vec8<T>::one(x + t * st + d) * inv : 0.f;
+            const uint32_t c = pack_e4m3(f, 0.f, 0.f, 0.f) & 0xffu;
+            o[p >> 2] = (o[p >> 2] & ~(0xffu << (8 * (p & 3)))) | c << (8 * (p & 3));
+          }
+          *(uint4*)dst = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+          for (int p = 0; p < 16; ++p) {
+            const int t = last[g * 16 + p];
+            if (t < 0) continue;
+            const float f = valid ? Vec8<T>::one(x + t * st + d) * inv : 0.f;
+            dst[p] = (uint8_t)pack_e4m3(f, 0.f, 0.f, 0.f);
+          }
+        }
+      }
+    }
+  }
+}
+
+int after_launch(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? GI_OK : hip_fail(e, what);
+}
+
+int log2_page(int page_size) {
+  for (int l = 4; l <= 8; ++l)
+    if (page_size == 1 << l) return l;
+  return -1;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+}  // namespace
+
+int launch_kv_slots(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* block_table, int max_pages,
+                    int64_t table_stride, const int32_t* free_pages, int n_free, const int32_t* free_used,
+                    int page_size, int64_t* slots, int64_t* positions, int n_tokens, int32_t* q_start,
+                    int32_t* seq_lens, int32_t* status, hipStream_t stream) {
+  if (B < 0 || max_pages < 0 || n_free < 0 || n_tokens < 0 || table_stride < max_pages)
+    return fail(GI_ERR_INVALID_ARG, "kv_slots: negative size, or table_stride < max_pages");
+  if (B > kMaxRequests) return fail(GI_ERR_UNSUPPORTED, "kv_slots: at most 8192 requests");
+  const int lp = log2_page(page_size);
+  if (lp < 0) return fail(GI_ERR_INVALID_ARG, "kv_slots: page_size must be 16, 32, 64, 128 or 256");
+  if (!free_used || !q_start || !status || (n_free > 0 && !free_pages) || (n_tokens > 0 && (!slots || !positions)) ||
+      (B > 0 && (!ctx_lens || !new_lens || !seq_lens || (max_pages > 0 && !block_table))))
+    return fail(GI_ERR_INVALID_ARG, "kv_slots: null pointer");
+  SlotArgs a{ctx_lens, new_lens, block_table, free_pages, free_used, slots,  positions, q_start,
+             seq_lens, status,   table_stride, B,         max_pages, n_free, lp,        n_tokens};
+  const int wgs = n_tokens > 0 ? (n_tokens - 1) / kSlotThreads + 1 : 1;
+  hipLaunchKernelGGL(kv_slots_kernel, dim3(wgs), dim3(kSlotThreads), (size_t)B * 2 * sizeof(int), stream, a);
+  return after_launch("kv_slots launch");
+}
+
+int launch_kv_append(const void* k, const void* v, int dtype, const int64_t* k_strides, const int64_t* v_strides,
+                     const int64_t* slots, int T, int Hk, int D, int page_size, int64_t num_pages, void* k_cache,
+                     void* v_cache, float* k_scale, float* v_scale, hipStream_t stream) {
+  if (dtype != GI_DTYPE_BF16 && dtype != GI_DTYPE_FP16 && dtype != GI_DTYPE_FP32)
+    return fail(GI_ERR_UNSUPPORTED, "kv_append: rows must be bf16, fp16 or fp32");
+  const int lp = log2_page(page_size);
+  if (lp < 0) return fail(GI_ERR_INVALID_ARG, "kv_append: page_size must be 16, 32, 64, 128 or 256");
+  if (T < 0 || Hk <= 0 || num_pages < 0 || D <= 0 || D % 8 || D > 1024)
+    return fail(GI_ERR_INVALID_ARG, "kv_append: T, num_pages >= 0, Hk > 0 and D a multiple of 8 up to 1024 required");
+  if (Hk > 65535) return fail(GI_ERR_UNSUPPORTED, "kv_append: at most 65535 kv heads");
+  if (T == 0 || num_pages == 0) return GI_OK;
+  if (!k || !v || !slots || !k_cache || !v_cache || !k_scale || !v_scale)
+    return fail(GI_ERR_INVALID_ARG, "kv_append: null pointer");
+  if (!aligned16(k_cache) || !aligned16(v_cache))
+    return fail(GI_ERR_INVALID_ARG, "kv_append: the cache must be 16-byte aligned");
+  AppendArgs a{};
+  a.x[0] = k;
+  a.x[1] = v;
+  a.st[0] = k_strides[0];
+  a.sh[0] = k_strides[1];
+  a.st[1] = v_strides[0];
+  a.sh[1] = v_strides[1];
+  a.slots = slots;
+  a.cache[0] = (uint8_t*)k_cache;
+  a.cache[1] = (uint8_t*)v_cache;
+  a.scale[0] = k_scale;
+  a.scale[1] = v_scale;
+  a.num_pages = num_pages;
+  a.T = T;
+  a.Hk = Hk;
+  a.D = D;
+  a.log_page = lp;
+  // a decode step's rows lie on pages of their own: a workgroup each; a
+  // prompt's lie on its pages in runs, and most workgroups would find nothing
+  a.per_wg = (int64_t)T * Hk > 8192 ? 16 : 1;
+  const int size = dtype == GI_DTYPE_FP32 ? 4 : 2;
+  bool vec = aligned16(k) && aligned16(v);
+  for (int i = 0; i < 2; ++i) vec = vec && a.st[i] * size % 16 == 0 && a.sh[i] * size % 16 == 0;
+  const dim3 grid((T - 1) / a.per_wg + 1, Hk, 2);
+#define GI_APPEND(T_)                                                                                        \
+  do {                                                                                                       \
+    if (vec) hipLaunchKernelGGL((kv_append_kernel<T_, true>), grid, dim3(kAppThreads), 0, stream, a);        \
+    else hipLaunchKernelGGL((kv_append_kernel<T_, false>), grid, dim3(kAppThreads), 0, stream, a);           \
+  } while (0)
+  if (dtype == GI_DTYPE_BF16) GI_APPEND(uint16_t);
+  else if (dtype == GI_DTYPE_FP16) GI_APPEND(_Float16);
+  else GI_APPEND(float);
+#undef GI_APPEND
+  return after_launch("kv_append launch");
+}
+
+}  // namespace gi

@@ -13,12 +13,19 @@ Reference entry points mirrored (GemmaInfer paths):
   softcapping         csrc/pybind.cpp:169-180 -> csrc/softcapping.cu:21-47
   rmsnorm             csrc/pybind.cpp:137-151 -> csrc/rmsnorm.cu:75-114
   fused_rope_inplace  csrc/pybind.cpp:153-167 -> csrc/rmsnorm.cu:166-231
+
+Without a native counterpart there (torch statements of
+gemmainfer/kernels/attention.py:135-277): attention over an 8-bit paged K/V
+cache -- kv_cache, kv_slots, rope_frequencies, rope_rows, kv_append,
+kv_attention.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 import threading
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -546,3 +553,275 @@ def fused_rope_inplace(q, k, cos, sin, position_ids):
         _ptr(q), _ptr(k) if has_k else None, _ptr(c), _ptr(sn), _ptr(pos), _DTYPE_CODE[q.dtype],
         b, hq, k.shape[1] if has_k else 0, s, d, q.stride(0), q.stride(1), q.stride(2),
         ks[0], ks[1], ks[2], _stream(dev)), "fused_rope_inplace")
+
+
+# ---------------------------------------------------------------------------
+# attention over an 8-bit paged K/V cache
+# ---------------------------------------------------------------------------
+class KVCache(NamedTuple):
+    """A pool of pages of e4m3 codes with one fp32 scale per page and kv head:
+    ``k`` [pages, Hk, page, D], ``v`` [pages, Hk, D, page] (transposed),
+    ``k_scale`` and ``v_scale`` [pages, Hk]; a value is code * scale."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+class KVSlots(NamedTuple):
+    """Where a step's rows go (``kv_slots``).  ``status`` is {free pages used
+    so far, pages that were lacking, rows dropped}."""
+    slots: torch.Tensor      # int64 [rows]
+    positions: torch.Tensor  # int64 [rows]
+    q_start: torch.Tensor    # int32 [B + 1]
+    seq_lens: torch.Tensor   # int32 [B]
+    status: torch.Tensor     # int32 [3]
+
+
+_PAGE_SIZES = (16, 32, 64, 128, 256)
+_HEAD_WIDTHS = (64, 128, 256, 512)
+
+
+def _launch_on(device: torch.device):
+    """Kernels are launched on the current device: make it the tensors' own."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def kv_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> KVCache:
+    """An empty cache.  ``page_size`` is 16, 32, 64, 128 or 256 tokens, ``head_dim``
+    64, 128, 256 or 512; a token takes 2 * kv_heads * head_dim bytes."""
+    _require(num_pages > 0 and kv_heads > 0, "kv_cache: num_pages and kv_heads must be positive")
+    _require(page_size in _PAGE_SIZES, f"kv_cache: page_size must be one of {_PAGE_SIZES}, got {page_size}")
+    _require(head_dim in _HEAD_WIDTHS, f"kv_cache: head_dim must be one of {_HEAD_WIDTHS}, got {head_dim}")
+    codes = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)  # noqa: E731
+    scale = lambda: torch.zeros((num_pages, kv_heads), dtype=torch.float32, device=device)  # noqa: E731
+    return KVCache(codes(num_pages, kv_heads, page_size, head_dim), codes(num_pages, kv_heads, head_dim, page_size),
+                   scale(), scale())
+
+
+def _cache_shape(cache, who):
+    k, v, ks, vs = cache
+    _require(k.dim() == 4 and v.dim() == 4, f"{who}: cache.k is [pages, Hk, page, D], cache.v [pages, Hk, D, page]")
+    pages, hk, page, d = k.shape
+    _require(v.shape == (pages, hk, d, page), f"{who}: cache.v must be {(pages, hk, d, page)}, got {tuple(v.shape)}")
+    _require(ks.shape == (pages, hk) and vs.shape == (pages, hk), f"{who}: cache scales must be [pages, Hk]")
+    _require(k.dtype == torch.float8_e4m3fn and v.dtype == torch.float8_e4m3fn,
+             f"{who}: cache.k and cache.v must be float8_e4m3fn", TypeError)
+    _require(ks.dtype == torch.float32 and vs.dtype == torch.float32, f"{who}: cache scales must be fp32", TypeError)
+    _require(k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous(),
+             f"{who}: the cache must be contiguous")
+    _require(page in _PAGE_SIZES, f"{who}: page size must be one of {_PAGE_SIZES}, got {page}")
+    return pages, hk, page, d
+
+
+def _ints(t, name, who, dtype, numel=None):
+    _require(t.dtype == dtype, f"{who}: {name} must be {dtype}, got {t.dtype}", TypeError)
+    _require(t.dim() == 1 and t.is_contiguous(), f"{who}: {name} must be a contiguous vector")
+    _require(numel is None or t.numel() == numel, f"{who}: {name} must have {numel} elements, got {t.numel()}")
+
+
+def _table(block_table, batch, who):
+    _require(block_table.dtype == torch.int32, f"{who}: block_table must be int32", TypeError)
+    _require(block_table.dim() == 2 and block_table.shape[0] == batch,
+             f"{who}: block_table must be [B={batch}, pages], got {tuple(block_table.shape)}")
+    cols = block_table.shape[1]
+    _require(cols == 0 or block_table.stride(1) == 1, f"{who}: block_table's rows must be contiguous")
+    _require(batch <= 1 or block_table.stride(0) >= cols, f"{who}: block_table's rows must not overlap")
+    return cols, max(block_table.stride(0), cols)
+
+
+def kv_slots(ctx_lens, new_lens, block_table, free_pages, free_used, page_size, num_rows) -> KVSlots:
+    """Places the new tokens of B requests on cache pages, on the device.
+
+    ``ctx_lens``/``new_lens`` int32 [B]: tokens in the cache, tokens to add.
+    ``block_table`` int32 [B, max_pages] is written where the step opens pages,
+    which come from ``free_pages`` (int32) behind the first ``free_used[0]`` of
+    them.  ``num_rows`` rows are laid out (the packed rows of q, k and v,
+    request after request); those behind the last request get slot -1 and
+    position 0.  A row without a page gets slot -1; ``status`` counts what was
+    lacking.  Pass ``status`` as the next step's ``free_used``."""
+    dev = _on_device(ctx_lens, new_lens, block_table, free_pages, free_used)
+    _require(ctx_lens.dim() == 1, "kv_slots: ctx_lens must be a vector")
+    b = ctx_lens.numel()
+    _ints(ctx_lens, "ctx_lens", "kv_slots", torch.int32)
+    _ints(new_lens, "new_lens", "kv_slots", torch.int32, b)
+    _ints(free_pages, "free_pages", "kv_slots", torch.int32)
+    _ints(free_used, "free_used", "kv_slots", torch.int32)
+    _require(free_used.numel() >= 1, "kv_slots: free_used must have an element")
+    _require(page_size in _PAGE_SIZES, f"kv_slots: page_size must be one of {_PAGE_SIZES}, got {page_size}")
+    _require(0 <= num_rows < 2 ** 31, f"kv_slots: num_rows must be in [0, 2^31), got {num_rows}")
+    cols, stride = _table(block_table, b, "kv_slots")
+    rows = torch.empty((2, num_rows), dtype=torch.int64, device=dev)
+    ints = torch.empty(2 * b + 4, dtype=torch.int32, device=dev)
+    r = KVSlots(rows[0], rows[1], ints[:b + 1], ints[b + 1:2 * b + 1], ints[2 * b + 1:])
+    with _launch_on(dev):
+        L.check(L.load().gi_kv_slots(
+            _ptr(ctx_lens), _ptr(new_lens), b, _ptr(block_table), cols, stride, _ptr(free_pages),
+            free_pages.numel(), _ptr(free_used), int(page_size), _ptr(r.slots), _ptr(r.positions), int(num_rows),
+            _ptr(r.q_start), _ptr(r.seq_lens), _ptr(r.status), _stream(dev)), "kv_slots")
+    return r
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
+                     original_len: int = 8192, fast: float = 32.0, slow: float = 1.0, device="cuda"):
+    """(inv_freq fp64 [rotary_dim / 2], mscale) for ``rope_rows``: base^(-2i / rotary_dim), and for long contexts
+
+    * ``scaling="linear"``: every frequency divided by ``factor``;
+    * ``scaling="ntk"``: base * factor^(d / (d - 2)), which leaves the fastest
+      frequency and divides the slowest by ``factor``;
+    * ``scaling="yarn"``: frequencies that turn more than ``fast`` times in
+      ``original_len`` tokens are left, those of fewer than ``slow`` turns are
+      divided by ``factor``, with a linear ramp over the turns between; mscale = 0.1 ln(factor) + 1.
+    """
+    _require(rotary_dim > 0 and rotary_dim % 2 == 0, f"rope_frequencies: rotary_dim must be even, got {rotary_dim}")
+    _require(scaling in (None, "linear", "ntk", "yarn"),
+             f"rope_frequencies: scaling must be None, 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    _require(base > 0 and factor >= 1, "rope_frequencies: base > 0 and factor >= 1 required")
+    if scaling == "ntk" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    f = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    mscale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        _require(fast > slow, "rope_frequencies: fast must be greater than slow")
+        turns = original_len * f / (2 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0, 1)
+        f = f / factor * (1 - keep) + f * keep
+        mscale = 0.1 * math.log(factor) + 1
+    return f.to(device), mscale
+
+
+def rope_rows(q, k, positions, inv_freq, *, interleaved: bool = False, mscale: float = 1.0, inplace: bool = False):
+    """Rotary embedding of packed rows q [T, Hq, D] and k [T, Hk, D] (or None) at
+    ``positions`` (int64 [T]); returns the rotated (q, k), which are q and k
+    themselves with ``inplace``.
+
+    ``inv_freq`` (fp64, on the device; ``rope_frequencies``) holds one frequency
+    per rotated pair: the first 2 * len(inv_freq) dimensions turn, pair i being
+    (i, i + len) or, ``interleaved``, (2i, 2i + 1); the others are kept.
+    ``mscale`` multiplies cos and sin."""
+    dev = _on_device(q, positions, inv_freq)
+    _require(q.dtype in _ACT_DTYPES, "rope_rows: bf16/fp16/fp32 only", TypeError)
+    _require(q.dim() == 3, f"rope_rows: q must be [T, Hq, D], got {tuple(q.shape)}")
+    t, hq, d = q.shape
+    _require(q.stride(2) == 1 or d == 1, "rope_rows: q's last dimension must be contiguous")
+    if k is not None:
+        _on_device(q, k)
+        _require(k.dim() == 3 and k.shape[0] == t and k.shape[2] == d and k.dtype == q.dtype,
+                 "rope_rows: k must be [T, Hk, D] like q")
+        _require(k.stride(2) == 1 or d == 1, "rope_rows: k's last dimension must be contiguous")
+    _ints(positions, "positions", "rope_rows", torch.int64, t)
+    _require(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(),
+             "rope_rows: inv_freq must be a contiguous fp64 vector", TypeError)
+    rot = 2 * inv_freq.numel()
+    _require(0 < rot <= d, f"rope_rows: {inv_freq.numel()} frequencies rotate {rot} of {d} dimensions")
+    if inplace:
+        qo, ko = q, k
+        for name, x in (("q", q), ("k", k)):
+            _require(x is None or x.numel() == 0 or all(s > 0 or n == 1 for s, n in zip(x.stride(), x.shape)),
+                     f"rope_rows: {name} has broadcast dimensions, which cannot be rotated in place")
+    else:
+        qo = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+        ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+    if t == 0:
+        return qo, ko
+    ks, kos = ((0, 0), (0, 0)) if k is None else (k.stride(), ko.stride())
+    with _launch_on(dev):
+        L.check(L.load().gi_rope_rows(
+            _ptr(q), _ptr(qo), _ptr(k), _ptr(ko), _ptr(positions), _ptr(inv_freq), _DTYPE_CODE[q.dtype], t, hq,
+            0 if k is None else k.shape[1], d, rot, int(bool(interleaved)), float(mscale), q.stride(0), q.stride(1),
+            qo.stride(0), qo.stride(1), ks[0], ks[1], kos[0], kos[1], _stream(dev)), "rope_rows")
+    return qo, ko
+
+
+def kv_append(k, v, slots, cache: KVCache) -> None:
+    """Stores rows k and v [T, Hk, D] (bf16/fp16/fp32) in the cache at ``slots``
+    (int64 [T]; negative ones, and those past the last page, are skipped).
+
+    The rows of one page must follow each other, as those of a request do; of
+    rows with the same slot the last one is stored.  Each page has one scale per head for K and one for V,
+    a power of two that grows as larger rows arrive (what the page holds is
+    then rounded to the new one); writing a page's first place starts the page
+    anew.  A row with an infinity or NaN makes its page's scale NaN until then."""
+    dev = _on_device(k, v, slots, *cache)
+    pages, hk, page, d = _cache_shape(cache, "kv_append")
+    _require(k.dtype in _ACT_DTYPES and v.dtype == k.dtype, "kv_append: k and v must be bf16, fp16 or fp32, alike",
+             TypeError)
+    _require(k.dim() == 3 and k.shape[1:] == (hk, d) and v.shape == k.shape,
+             f"kv_append: k and v must be [T, {hk}, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    _require(k.stride(2) == 1 and v.stride(2) == 1, "kv_append: the last dimension of k and v must be contiguous")
+    t = k.shape[0]
+    _ints(slots, "slots", "kv_append", torch.int64, t)
+    with _launch_on(dev):
+        L.check(L.load().gi_kv_append(
+            _ptr(k), _ptr(v), _DTYPE_CODE[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1), _ptr(slots),
+            t, hk, d, page, pages, _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale),
+            _stream(dev)), "kv_append")
+
+
+def _rows_aligned(x):
+    return x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.data_ptr() % 16 == 0
+
+
+def _overlap(x, y):
+    """Whether the bytes that two tensors span meet (a tensor's own gaps count as its)."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a, b), (c, d) = span(x), span(y)
+    return x.numel() > 0 and y.numel() > 0 and a < d and c < b
+
+
+def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scale: Optional[float] = None,
+                 window: int = 0, out=None):
+    """Causal attention of packed query rows q [T, Hq, D] (bf16 or fp16) over the
+    cache; returns [T, Hq, D].
+
+    Rows ``q_start[b]`` to ``q_start[b + 1]`` (int32 [B + 1]; None: one row a
+    request) are the last tokens of request b, which has ``seq_lens[b]`` (int32)
+    tokens in the pages ``block_table[b]`` names, those rows' own among them.  A
+    row sees the tokens up to its own, with ``window`` > 0 the last ``window`` of
+    them; one that sees none gets zeros.  ``scale`` defaults to D ** -0.5.  Query
+    head h reads kv head h // (Hq // Hk).  Rows behind the last request are not
+    computed: they keep what ``out`` holds, and are unspecified without it.  A
+    row that sees a token without a page (outside the cache, or past the table) gets NaN."""
+    dev = _on_device(q, block_table, seq_lens, *cache)
+    pages, hk, page, d = _cache_shape(cache, "kv_attention")
+    _require(q.dtype in (torch.bfloat16, torch.float16), f"kv_attention: q must be bf16 or fp16, got {q.dtype}",
+             TypeError)
+    _require(q.dim() == 3 and q.shape[2] == d and q.shape[1] % hk == 0 and q.shape[1] > 0,
+             f"kv_attention: q must be [T, a multiple of {hk}, {d}], got {tuple(q.shape)}")
+    _require(d in _HEAD_WIDTHS, f"kv_attention: head width must be one of {_HEAD_WIDTHS}, got {d}")
+    t, hq, _ = q.shape
+    _require(seq_lens.dim() == 1, "kv_attention: seq_lens must be a vector")
+    b = seq_lens.numel()
+    _ints(seq_lens, "seq_lens", "kv_attention", torch.int32)
+    cols, stride = _table(block_table, b, "kv_attention")
+    if q_start is None:
+        _require(t == b, f"kv_attention: without q_start there is one row a request: {t} rows, {b} requests")
+    else:
+        _on_device(q, q_start)
+        _ints(q_start, "q_start", "kv_attention", torch.int32, b + 1)
+    _require(int(window) >= 0, f"kv_attention: window must be >= 0 (0: none), got {window}")
+    if out is None:
+        out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+    else:
+        _on_device(q, out)
+        _require(out.shape == q.shape and out.dtype == q.dtype and _rows_aligned(out),
+                 "kv_attention: out must be like q, its rows contiguous and 16-byte aligned")
+        _require(not _overlap(q, out), "kv_attention: out must not overlap q")
+    if t == 0 or b == 0:
+        return out
+    if not _rows_aligned(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    lib = L.load()
+    nbytes = lib.gi_kv_attention_workspace_bytes(t, b, hq, hk, d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with _launch_on(dev):
+        L.check(lib.gi_kv_attention(
+            _ptr(q), _DTYPE_CODE[q.dtype], q.stride(0), q.stride(1), _ptr(cache.k), _ptr(cache.v),
+            _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(block_table), cols, stride, _ptr(seq_lens),
+            _ptr(q_start), _ptr(out), out.stride(0), out.stride(1), t, b, hq, hk, d, page, pages,
+            float(d ** -0.5 if scale is None else scale), int(window), _ptr(ws), nbytes, _stream(dev)),
+            "kv_attention")
+    return out

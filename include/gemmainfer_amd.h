@@ -339,6 +339,95 @@ int gi_rope_inplace(void* q, void* k, const void* cos_t, const void* sin_t,
                     int64_t q_sb, int64_t q_sh, int64_t q_ss,
                     int64_t k_sb, int64_t k_sh, int64_t k_ss, void* stream);
 
+/* ---- attention over an 8-bit paged K/V cache ------------------------------
+ * The stretch of a decoder layer between the q/k/v projections and the output
+ * projection, on packed rows: row t of q/k/v is one token of one request, the
+ * rows of a request follow each other (the reference keeps a dense bf16 cache
+ * per sequence and calls torch's attention, gemmainfer/kernels/attention.py:
+ * 135-277; no native counterpart there).
+ *
+ * The cache is a pool of pages of page_size tokens (16, 32, 64, 128 or 256):
+ *   k_cache  e4m3 (OCP) [num_pages, Hk, page_size, D]
+ *   v_cache  e4m3       [num_pages, Hk, D, page_size]   (transposed)
+ *   k_scale, v_scale  fp32 [num_pages, Hk];  value = code * scale
+ * block_table int32 [B, max_pages] (rows table_stride apart): the page of
+ * tokens [j*page_size, (j+1)*page_size) of request b is block_table[b][j].
+ * A token's slot is page * page_size + place in the page.                   */
+
+/* Rotary embedding of packed rows: q [T, Hq, D], k [T, Hk, D] (k may be NULL),
+ * last dimension contiguous, row/head strides in elements, into q_out/k_out
+ * (which may be q/k with the same strides: in place).  Pair i of the first
+ * rotary_dim dimensions, (i, i + rotary_dim/2) or, interleaved, (2i, 2i+1),
+ * turns by positions[t] * inv_freq[i]; the angle is formed and reduced in fp64.
+ * mscale multiplies cos and sin (1 unless the frequencies are scaled for long
+ * contexts in a way that asks for it).  Dimensions from rotary_dim on are
+ * copied.  inv_freq fp64 [rotary_dim/2], positions int64 [T].
+ * bf16/fp16/fp32; rotary_dim even, at most D and 1024.                      */
+int gi_rope_rows(const void* q, void* q_out, const void* k, void* k_out,
+                 const int64_t* positions, const double* inv_freq, int dtype,
+                 int T, int Hq, int Hk, int D, int rotary_dim, int interleaved, float mscale,
+                 int64_t q_st, int64_t q_sh, int64_t qo_st, int64_t qo_sh,
+                 int64_t k_st, int64_t k_sh, int64_t ko_st, int64_t ko_sh, void* stream);
+
+/* Places the new tokens of B requests (ctx_lens[b] tokens in the cache,
+ * new_lens[b] to add; negative counts as 0) on pages:
+ *   q_start int32 [B+1]  first row of each request in the packed rows
+ *   seq_lens int32 [B]   tokens after the step
+ *   slots, positions int64 [n_tokens]  of each row; rows behind the last
+ *                        request get slot -1 and position 0
+ *   block_table          entries of the pages that the step opens are written
+ * Pages are taken from free_pages[free_used[0] ...] in the order of the
+ * requests; none is taken for a page that holds tokens already.  status int32
+ * [3] = {free_used after the step, pages that were lacking (the list was used
+ * up, or the request needs more than max_pages), rows past n_tokens that were
+ * dropped}.  A row whose page is lacking gets slot -1, and its table entry -1.
+ * status may serve as the next step's free_used, but not as this one's.
+ * B <= 8192.                                                                */
+int gi_kv_slots(const int32_t* ctx_lens, const int32_t* new_lens, int B,
+                int32_t* block_table, int max_pages, int64_t table_stride,
+                const int32_t* free_pages, int n_free, const int32_t* free_used, int page_size,
+                int64_t* slots, int64_t* positions, int n_tokens,
+                int32_t* q_start, int32_t* seq_lens, int32_t* status, void* stream);
+
+/* Writes rows of K and V ([T, Hk, D], last dimension contiguous, strides in
+ * elements; bf16, fp16 or fp32) into their slots.  Slots that are negative or
+ * past the last page are skipped.  The rows of one page must follow each other
+ * in the call (those of a request do); of rows with the same slot the last one
+ * is stored.  A page's scale (per head, K and V apart) is the smallest power of two, at
+ * least 2^-40, that brings its largest value to at most 448.  Writing a page's
+ * first place starts the page anew, with the scale of the rows of this call;
+ * otherwise the scale only grows, and what the page holds is rounded to the
+ * new scale.  A page that is given an infinity, a NaN or a value over 448 *
+ * 2^40 gets a NaN scale (attention that sees one of its tokens returns NaN)
+ * until it is started anew.  D a multiple of 8 up to 1024.                  */
+int gi_kv_append(const void* k, const void* v, int dtype,
+                 int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                 const int64_t* slots, int T, int Hk, int D, int page_size, int64_t num_pages,
+                 void* k_cache, void* v_cache, float* k_scale, float* v_scale, void* stream);
+
+/* out[t, h] = softmax(scale * q[t, h] . K) V over the tokens that row t sees.
+ * Rows q_start[b] ... q_start[b+1]-1 belong to request b (NULL: one row a
+ * request, T == B) and are its last ones: with n rows, row i is at position
+ * seq_lens[b] - n + i and sees tokens up to it, and with window > 0 only the
+ * last `window` of those.  Head h reads kv head h / (Hq / Hk).  A row that
+ * sees nothing gets zeros; rows behind q_start[B] are not touched.  A row that
+ * sees a token whose page is outside [0, num_pages), or whose request is longer
+ * than its table, gets NaN.  Scales of pages must be positive.
+ * q, out bf16 or fp16 [T, Hq, D], last dimension contiguous, other strides
+ * multiples of 8 elements, 16-byte aligned; D 64, 128, 256 or 512; fp32 sums
+ * and softmax statistics.  Deterministic.  The workspace is scratch: it needs
+ * no initial value and holds nothing between calls.                         */
+size_t gi_kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D);
+int gi_kv_attention(const void* q, int dtype, int64_t q_st, int64_t q_sh,
+                    const void* k_cache, const void* v_cache,
+                    const float* k_scale, const float* v_scale,
+                    const int32_t* block_table, int max_pages, int64_t table_stride,
+                    const int32_t* seq_lens, const int32_t* q_start,
+                    void* out, int64_t o_st, int64_t o_sh,
+                    int T, int B, int Hq, int Hk, int D, int page_size, int64_t num_pages,
+                    float scale, int window,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

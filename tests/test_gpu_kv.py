@@ -1,0 +1,669 @@
+"""Slots, rotary rows, append and attention over the 8-bit paged cache, against
+the float64 oracle (oracle/kv_oracle.py), at the sizes and masks where they can go wrong."""
+import random
+
+import pytest
+import torch
+
+from gemmainfer_amd import _lib as L
+from gemmainfer_amd import ops, synth
+from oracle import kv_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# ---------------------------------------------------------------------------
+# slots
+# ---------------------------------------------------------------------------
+def _check_slots(ctx, new, page, rows, cols, n_free, used, pad=0):
+    rng = random.Random(len(ctx) * 7 + rows)
+    ids = list(range(3, 3 + 4 * (n_free + sum(-(-max(c, 0) // page) for c in ctx)) + 50))
+    rng.shuffle(ids)
+    table = [[ids.pop() if j < -(-c // page) else -1 for j in range(cols)] for c in ctx]
+    free = ids[:n_free]
+    wide = torch.full((len(ctx), cols + pad), -7, dtype=torch.int32)
+    if ctx and cols:
+        wide[:, :cols] = torch.tensor(table, dtype=torch.int32)
+    wide = wide.to(DEV)
+    free_t, used_t = _i32(free), _i32([used])
+    r = ops.kv_slots(_i32(ctx), _i32(new), wide[:, :cols], free_t, used_t, page, rows)
+    s, p, start, lens, status, want = O.slots(ctx, new, table, free, used, page, rows)
+    assert r.slots.tolist() == s
+    assert r.positions.tolist() == p
+    assert r.q_start.tolist() == start
+    assert r.seq_lens.tolist() == lens
+    assert r.status.tolist() == status
+    assert wide[:, :cols].tolist() == want
+    assert (wide[:, cols:] == -7).all()
+    assert free_t.tolist() == free and used_t.tolist() == [used]
+
+
+@pytest.mark.parametrize("b,page", [(1, 16), (3, 32), (64, 16), (257, 64), (1000, 256)])
+def test_slots_ragged(b, page):
+    rng = random.Random(b)
+    ctx = [rng.choice([0, 1, page - 1, page, page + 1, rng.randint(0, 900)]) for _ in range(b)]
+    new = [rng.choice([0, 1, 1, page, page + 1, rng.randint(0, 70)]) for _ in range(b)]
+    need = sum(-(-(c + n) // page) - -(-c // page) for c, n in zip(ctx, new))
+    cols = max(-(-(c + n) // page) for c, n in zip(ctx, new)) + 1
+    _check_slots(ctx, new, page, sum(new) + 5, cols, need + 4, 2, pad=3)
+
+
+@pytest.mark.parametrize("ctx,new,rows,cols,n_free,used", [
+    ([], [], 0, 4, 3, 0),                              # no requests, no rows
+    ([], [], 300, 0, 0, 0),                            # only padding
+    ([5, 9], [0, 0], 7, 2, 1, 0),                      # nothing to add
+    ([0, 0, 16], [40, 1, 1], 20, 4, 9, 0),             # rows dropped inside a request
+    ([0, 30, 16], [40, 10, 30], 80, 4, 2, 0),          # the list runs out inside a request
+    ([0, 30], [40, 10], 50, 4, 2, 2),                  # none left
+    ([0, 30], [40, 10], 50, 4, 2, 9),                  # more used than there are
+    ([0, 30], [200, 10], 210, 4, 40, 1),               # a request longer than its table
+    ([70], [3], 3, 4, 5, 0),                           # ... already before the step
+    ([-4, 3], [5, -2], 9, 2, 3, 0),                    # negative lengths count as none
+    ([0], [5000], 5000, 320, 313, 0),                  # one prompt over many workgroups
+])
+def test_slots_edges(ctx, new, rows, cols, n_free, used):
+    _check_slots(ctx, new, 16, rows, cols, n_free, used)
+
+
+def test_slots_many_requests_and_status_chain():
+    b = 8192
+    table = torch.full((b, 3), -1, dtype=torch.int32, device=DEV)
+    free = torch.arange(2 * b, dtype=torch.int32, device=DEV)
+    one = torch.ones(b, dtype=torch.int32, device=DEV)
+    r = ops.kv_slots(torch.zeros_like(one), one, table, free, _i32([0]), 16, b)
+    assert torch.equal(r.slots, torch.arange(b, device=DEV) * 16)
+    r = ops.kv_slots(r.seq_lens, 15 * one, table, free, r.status, 16, 15 * b)
+    assert r.status.tolist() == [b, 0, 0]
+    r = ops.kv_slots(r.seq_lens, one, table, free, r.status, 16, b)
+    assert r.status.tolist() == [2 * b, 0, 0]
+    assert torch.equal(r.slots, (torch.arange(b, device=DEV) + b) * 16)
+    r = ops.kv_slots(r.seq_lens, 16 * one, table, free, r.status, 16, 16 * b)
+    assert r.status.tolist() == [2 * b, b, 0]          # the last of each request's 16 rows has no page
+    assert (r.slots.view(b, 16)[:, 15] == -1).all() and (r.slots.view(b, 16)[:, :15] >= 0).all()
+
+
+# ---------------------------------------------------------------------------
+# rope
+# ---------------------------------------------------------------------------
+HALF = {BF16: 2.0 ** -8, FP16: 2.0 ** -11, FP32: 2.0 ** -24}  # half a step, relative (finfo.eps / 2)
+
+
+def _check_rope(got, x, pos, freq, inter, mscale):
+    # the reduced angle is off by 2^-26 turns (4.7e-8 rad half step, 9.4e-8 with the fp64 product's
+    # rounding at these positions), cos and sin by a few units of 2^-24, two products and a sum by three
+    # roundings: under 2^-20 (9.5e-7) of |x1| + |x2| together, then half a step of the stored type
+    y, size = O.rope(x, pos, freq, inter, mscale)
+    bound = HALF[x.dtype] * y.abs() + 2.0 ** -20 * mscale * size
+    bound += (2.0 ** -25 if x.dtype == FP16 else 0.0)  # fp16's subnormal half step
+    assert ((got.double() - y).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("t,hq,hk,d,rot,inter", [
+    (1, 16, 2, 512, 128, False), (3, 4, 1, 64, 64, True), (257, 16, 8, 256, 256, False), (5, 3, 3, 128, 48, True),
+    (7, 2, 1, 80, 40, False), (2, 5, 2, 30, 6, True), (4, 1, 1, 66, 66, False), (2, 1, 1, 1024, 1024, True),
+    (6, 2, 2, 64, 24, True), (6, 2, 2, 64, 24, False)])
+def test_rope_rows(dtype, t, hq, hk, d, rot, inter):
+    g = _gen(t * d)
+    q, k = torch.randn(t, hq, d, generator=g).to(dtype), torch.randn(t, hk, d, generator=g).to(dtype)
+    pos = torch.randint(0, 1 << 20, (t,), generator=g)
+    freq, mscale = ops.rope_frequencies(rot, 1e4, scaling="yarn", factor=4.0, device=DEV)
+    qd, kd = q.to(DEV), k.to(DEV)
+    qo, ko = ops.rope_rows(qd, kd, pos.to(DEV), freq, interleaved=inter, mscale=mscale)
+    assert torch.equal(qd.cpu(), q) and torch.equal(kd.cpu(), k)
+    _check_rope(qo.cpu(), q, pos, freq.cpu(), inter, mscale)
+    _check_rope(ko.cpu(), k, pos, freq.cpu(), inter, mscale)
+    # in place, on slices of a wider tensor: the same bits, and nothing around them
+    wide = torch.full((t, hq + hk + 1, d + 8), 3.0, dtype=dtype, device=DEV)
+    qs, ks = wide[:, :hq, :d], wide[:, hq:hq + hk, :d]
+    qs.copy_(qd), ks.copy_(kd)
+    a, b = ops.rope_rows(qs, ks, pos.to(DEV), freq, interleaved=inter, mscale=mscale, inplace=True)
+    assert a is qs and b is ks
+    assert torch.equal(qs, qo) and torch.equal(ks, ko)
+    assert (wide[:, hq + hk:] == 3).all() and (wide[..., d:] == 3).all()
+    # heads before rows, an odd offset, no k
+    buf = torch.empty(hq * t * d + 1, dtype=dtype, device=DEV)[1:].view(hq, t, d).transpose(0, 1)
+    buf.copy_(qd)
+    only, none = ops.rope_rows(buf, None, pos.to(DEV), freq, interleaved=inter, mscale=mscale)
+    assert none is None and torch.equal(only, qo)
+
+
+def test_rope_matches_the_table_form():
+    """fused_rope_inplace with tables of the same angles: equal to a rounding of each."""
+    t, d = 33, 256
+    q = torch.randn(t, 4, d, generator=_gen(1)).to(DEV)
+    freq, _ = ops.rope_frequencies(d, device=DEV)
+    ang = torch.arange(t, device=DEV, dtype=torch.float64)[:, None] * freq
+    ang = torch.cat([ang, ang], -1)
+    ref = q.transpose(0, 1)[None].clone()
+    ops.fused_rope_inplace(ref, None, ang.cos().float(), ang.sin().float(), torch.arange(t, device=DEV)[None])
+    out, _ = ops.rope_rows(q, None, torch.arange(t, device=DEV), freq)
+    assert ((ref[0].transpose(0, 1) - out).abs() <= 2.0 ** -19 * (q.abs() + q.abs().roll(d // 2, -1))).all()
+
+
+def test_rope_empty_and_negative_positions():
+    freq, _ = ops.rope_frequencies(64, device=DEV)
+    e = torch.empty(0, 2, 64, dtype=BF16, device=DEV)
+    assert ops.rope_rows(e, e, torch.empty(0, dtype=torch.int64, device=DEV), freq)[0].shape == (0, 2, 64)
+    q, pos = torch.randn(3, 2, 64, generator=_gen(2)), torch.tensor([-5, 0, -100000])
+    got, _ = ops.rope_rows(q.to(DEV), None, pos.to(DEV), freq)
+    _check_rope(got.cpu(), q, pos, freq.cpu(), False, 1.0)
+
+
+def test_rope_frequency_scaling():
+    base, _ = ops.rope_frequencies(128, 5e5, device="cpu")
+    lin, m = ops.rope_frequencies(128, 5e5, scaling="linear", factor=8, device="cpu")
+    assert torch.equal(lin, base / 8) and m == 1.0
+    ntk, _ = ops.rope_frequencies(128, 5e5, scaling="ntk", factor=8, device="cpu")
+    assert ntk[0] == 1 and abs(float(ntk[-1] / base[-1]) - 1 / 8) < 1e-12
+    yarn, m = ops.rope_frequencies(128, 5e5, scaling="yarn", factor=8, original_len=4096, device="cpu")
+    turns = 4096 * base / (2 * torch.pi)
+    assert torch.equal(yarn[turns > 32], base[turns > 32])
+    assert torch.allclose(yarn[turns < 1], base[turns < 1] / 8, rtol=1e-15, atol=0) and m > 1
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+def _filled(pages, hk, page, d, seed, spread=1.0):
+    """A cache (CPU tensors) of random pages whose sizes differ by page and head."""
+    g = _gen(seed)
+    r = []
+    for shape in ((pages, hk, page, d), (pages, hk, d, page)):
+        x = torch.randn(shape, generator=g) * torch.exp2(spread * torch.randn(pages, hk, 1, 1, generator=g))
+        s = torch.tensor([[O.page_scale(float(x[p, h].abs().max())) for h in range(hk)] for p in range(pages)])
+        r.append(((x / s[:, :, None, None]).to(O.E4M3), s))
+    return ops.KVCache(r[0][0], r[1][0], r[0][1], r[1][1])
+
+
+def _to(cache, dev):
+    return ops.KVCache(*[t.to(dev).clone() for t in cache])
+
+
+def _same_cache(got, want):
+    for name, x, y in zip(got._fields, got, want):
+        x = x.cpu()
+        if x.dtype == O.E4M3:
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), name
+        else:
+            assert torch.equal(torch.isnan(x), torch.isnan(y)) and torch.equal(x[~torch.isnan(x)], y[~torch.isnan(y)]), name
+
+
+def _check_append(cache, k, v, slots):
+    dev = _to(cache, DEV)
+    ops.kv_append(k.to(DEV), v.to(DEV), torch.tensor(slots, dtype=torch.int64, device=DEV), dev)
+    want = O.append(k, v, slots, cache)
+    _same_cache(dev, want)
+    return ops.KVCache(*want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("page,d,hk", [(16, 64, 1), (32, 128, 3), (64, 256, 2), (128, 512, 1), (256, 64, 2)])
+def test_append_runs(dtype, page, d, hk):
+    """Rows into the middle of pages, over page ends, whole pages, lone rows; small rows and ones
+    that raise the scale; then the same call again changes nothing."""
+    pages = 9
+    cache = _filled(pages, hk, page, d, seed=page)
+    g = _gen(d)
+    slots = [3 * page + page - 2, 3 * page + page - 1, *range(5 * page, 6 * page), 7 * page, 7 * page + 1,
+             *range(1 * page + 5, 1 * page + page - 1), 8 * page + 3, 2 * page + page // 2]
+    t = len(slots)
+    size = torch.exp2(2 * torch.randn(t, hk, 1, generator=g))
+    k = (torch.randn(t, hk, d, generator=g) * size).to(dtype)
+    v = (torch.randn(t, hk, d, generator=g) * size).to(dtype)
+    once = _check_append(cache, k, v, slots)
+    again = _check_append(once, k, v, slots)
+    _same_cache(_to(again, "cpu"), once)
+
+
+@pytest.mark.parametrize("t,hk,page", [(1, 1, 16), (700, 2, 16), (300, 40, 64)])
+def test_append_prompt_and_decode_sized_grids(t, hk, page):
+    """Both grid forms (a workgroup for each row, for sixteen rows), and runs cut by their borders."""
+    pages = -(-t // page) + 3
+    cache = ops.KVCache(*[x.cpu() for x in ops.kv_cache(pages, hk, page, 64, DEV)])
+    k, v = torch.randn(t, hk, 64, generator=_gen(t)).to(BF16), torch.randn(t, hk, 64, generator=_gen(t + 1)).to(BF16)
+    first = [2 * page + i for i in range(t)]
+    cache = _check_append(cache, k, v, first)
+    n = max(1, t // 2)
+    _check_append(cache, 3 * k[:n], 3 * v[:n], [s + 5 for s in first[:n]])
+
+
+def test_append_skips_duplicates_and_bad_slots():
+    page, d = 16, 64
+    cache = _filled(6, 2, page, d, seed=4)
+    slots = [-1, -5, 17, 18, 17, 17, -1, 6 * page, 6 * page + 3, 1 << 40, 33, 33, 33, -(1 << 40), 95, -1]
+    k = torch.randn(len(slots), 2, d, generator=_gen(1)).to(BF16)
+    k[3] *= 300  # the larger of two rows that go to different places
+    k[2] *= 1e6  # a row that another one replaces: it does not count
+    _check_append(cache, k, k.flip(0), slots)
+    # padding that names place 0 over and over: one row stays
+    _check_append(cache, k, k.flip(0), [0] * len(slots))
+    many = torch.randn(900, 2, d, generator=_gen(2)).to(BF16)
+    _check_append(cache, many, many, [3 * page + i % 5 for i in range(900)])
+    e = torch.empty(0, 2, d, dtype=BF16)
+    _check_append(cache, e, e, [])
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan"), 3e38, 448.0 * 2 ** 40, 2.0 ** -133, 0.0])
+def test_append_extreme_values(value):
+    page, d = 16, 64
+    cache = _filled(4, 2, page, d, seed=6)
+    k, v = torch.randn(3, 2, d, generator=_gen(3)).to(BF16), torch.zeros(3, 2, d, dtype=BF16)
+    k[1, 1, 7] = v[2, 0, 3] = value
+    cache = _check_append(cache, k, v, [17, 18, 40])
+    # a page without a scale keeps none while it is added to ...
+    cache = _check_append(cache, torch.ones_like(k), torch.ones_like(k), [19, 20, 41])
+    # ... until its first place is written
+    cache = _check_append(cache, torch.ones_like(k), torch.ones_like(k), [16, 17, 32])
+    assert not torch.isnan(cache.k_scale).any() and not torch.isnan(cache.v_scale).any()
+
+
+def test_append_rounds_and_rescales_every_code():
+    """Every e4m3 code moves to scales 1, 2, 4, ... 512 times as large, and every border between
+    two codes is rounded, as the definition says."""
+    page, d = 32, 256
+    codes = torch.arange(256, dtype=torch.uint8)
+    codes[127] = codes[255] = 0  # NaN codes are never written
+    cache = ops.KVCache(*[x.cpu() for x in ops.kv_cache(12, 1, page, d, DEV)])
+    cache.k.view(torch.uint8)[:, 0, 3] = codes
+    cache.v.view(torch.uint8)[:, 0, :, 3] = codes
+    cache.k_scale.fill_(2.0), cache.v_scale.fill_(0.25)
+    for e in range(11):
+        x = torch.zeros(1, 1, d, dtype=FP32)
+        x[0, 0, 0] = 448.0 * 2 ** e
+        _check_append(cache, x, x, [e * page + 9])
+    values = torch.unique(codes.view(O.E4M3).double())
+    mid = (values[1:] + values[:-1]) / 2
+    x = torch.cat([mid, mid * (1 + 2.0 ** -20), mid * (1 - 2.0 ** -20), values, values[:4]]).float()
+    x = torch.cat([x, torch.zeros(-len(x) % d)]).view(-1, 1, d)
+    x[:, 0, -1] = 448.0
+    _check_append(cache, x, x, list(range(2 * page, 2 * page + x.shape[0])))
+
+
+def test_append_strided_rows():
+    page, d, hk, t = 16, 128, 2, 21
+    cache = _filled(5, hk, page, d, seed=8)
+    qkv = torch.randn(t, 7 * d + 3, generator=_gen(5)).to(BF16)
+    slots = list(range(page + 3, page + 3 + t))
+    want = O.append(qkv[:, 3 * d:5 * d].reshape(t, hk, d), qkv[:, 5 * d + 3:7 * d + 3].reshape(t, hk, d), slots, cache)
+    on = qkv.to(DEV)
+    dev = _to(cache, DEV)
+    s = torch.tensor(slots, device=DEV)
+    ops.kv_append(on[:, 3 * d:5 * d].unflatten(1, (hk, d)), on[:, 5 * d + 3:].unflatten(1, (hk, d)), s, dev)
+    _same_cache(dev, want)
+    # heads before rows
+    dev = _to(cache, DEV)
+    k, v = on[:, 3 * d:5 * d].unflatten(1, (hk, d)), on[:, 5 * d + 3:].unflatten(1, (hk, d))
+    ops.kv_append(k.transpose(0, 1).contiguous().transpose(0, 1), v.transpose(0, 1).contiguous().transpose(0, 1), s, dev)
+    _same_cache(dev, want)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def _setup(lens, rows, hk, page, d, seed, spread=1.0, extra=2):
+    """A cache on the CPU, its table (entries behind a request's pages lead nowhere), q_start."""
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + extra
+    cache = _filled(pages, hk, page, d, seed, spread)
+    ids = list(range(pages))
+    random.Random(seed).shuffle(ids)
+    cols = max(need, default=0) + 1
+    table = [[ids.pop() if c < n else -1 for c in range(cols)] for n in need]
+    start = [0]
+    for r in rows:
+        start.append(start[-1] + r)
+    return cache, table, start
+
+
+def _check_out(got, ref, weighted, spread, d, tokens):
+    """Errors of the kernel: a score is an fp32 sum of D exact products and three more roundings, in
+    the exponent's unit (1/ln 2) beside log2 of a scale (|.| <= 40): e = (D + 8) 2^-24 (spread + 28); weights
+    are rounded to fp16 (2^-11; under 2^-21 of the largest to a step of 2^-25 / 2^7 of it) and so
+    are off by w = 2^-11 + 2 e together with the fp32 sums of the weights (tokens 2^-24, and of the
+    products: the same); the result is stored in half a step."""
+    e = (d + 8) * 2.0 ** -24 * (spread + 28)
+    w = 2.0 ** -11 + 2 * e + 2 * tokens * 2.0 ** -24
+    bound = HALF[got.dtype] * ref.abs() + (1 + HALF[got.dtype]) * w * weighted + tokens * 2.0 ** -31 * weighted.amax()
+    bound += 2.0 ** -24 if got.dtype == FP16 else 0.0
+    err = (got.cpu().double() - ref).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= bound).all(), f"{(err - bound).max()} over, {(err / bound.clamp(min=1e-30)).max()} of the bound"
+
+
+def _check_attention(lens, rows, hq, hk, page, d, dtype, window=0, seed=0, decode=False, scale=None, spread=1.0,
+                     q_size=2.0):
+    cache, table, start = _setup(lens, rows, hk, page, d, seed, spread)
+    q = (q_size * torch.randn(start[-1], hq, d, generator=_gen(seed + 1))).to(dtype)
+    dev = _to(cache, DEV)
+    got = ops.kv_attention(q.to(DEV), dev, _i32(table), _i32(lens), None if decode else _i32(start), scale=scale,
+                           window=window)
+    ref, weighted, size = O.attention(q, cache, table, lens, start, d ** -0.5 if scale is None else scale, window)
+    _check_out(got, ref, weighted, size, d, max(lens))
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("hq,hk,d,page", [(16, 8, 256, 16), (16, 2, 512, 64), (32, 8, 128, 32), (12, 4, 64, 128),
+                                          (7, 1, 64, 256), (5, 5, 128, 16), (40, 1, 256, 64)])
+def test_attention_decode(dtype, hq, hk, d, page):
+    """One row a request: every length around a group of 16, a unit of 64, a page; a long one beside."""
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 127, 129, 255, 257, 1000, 0, 333]
+    _check_attention(lens, [1] * len(lens), hq, hk, page, d, dtype, seed=d + page, decode=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("hq,hk,d,page", [(16, 8, 256, 16), (16, 2, 512, 32), (8, 2, 128, 64), (3, 1, 64, 16)])
+@pytest.mark.parametrize("window", [0, 1, 17, 64, 100])
+def test_attention_ragged_rows(dtype, hq, hk, d, page, window):
+    """Prompts, chunks onto a context, verify rows, no rows, rows that see nothing, with windows."""
+    lens = [40, 300, 7, 64, 0, 129, 3, 90]
+    rows = [40, 33, 7, 1, 0, 8, 5, 0]
+    got = _check_attention(lens, rows, hq, hk, page, d, dtype, window, seed=window + d)
+    assert (got[40 + 33 + 7 + 1 + 8:40 + 33 + 7 + 1 + 8 + 2] == 0).all()  # request of 3 tokens, 5 rows
+
+
+@pytest.mark.parametrize("rows,hq,hk,d", [(3, 16, 8, 256), (10, 16, 8, 256), (40, 16, 8, 256), (5, 16, 2, 512),
+                                          (20, 16, 2, 512), (70, 4, 4, 64), (30, 4, 4, 128), (100, 4, 4, 128)])
+def test_attention_row_tiles(rows, hq, hk, d):
+    """Each count of column tiles, cut and whole."""
+    _check_attention([rows + 111, rows], [rows, rows], hq, hk, 32, d, BF16, seed=rows)
+
+
+@pytest.mark.parametrize("b", [65, 130, 300])
+def test_attention_many_requests(b):
+    rng = random.Random(b)
+    lens = [rng.choice([0, 1, 5, 60, 100]) for _ in range(b)]
+    _check_attention(lens, [1] * b, 2, 1, 16, 64, BF16, seed=b, decode=True)
+    rows = [rng.choice([0, 1, 2]) for _ in range(b)]
+    _check_attention([n + r for n, r in zip(lens, rows)], rows, 2, 1, 16, 64, BF16, seed=b)
+
+
+@pytest.mark.parametrize("hq,hk,d,rows", [(16, 8, 256, 1), (16, 2, 512, 1), (4, 2, 64, 3), (8, 1, 128, 40)])
+def test_attention_long_axis_is_cut_and_joined(hq, hk, d, rows):
+    """A context over many workgroups: their partial sums, with sizes that differ from page to page."""
+    _check_attention([9001], [rows], hq, hk, 64, d, BF16, seed=rows, spread=3.0)
+
+
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_peaked_and_flat(window):
+    """Weights of one token, scores that run away late, and a scale of 0 (plain means)."""
+    for scale, size in ((1.0, 8.0), (0.0, 1.0), (-0.5, 2.0)):
+        _check_attention([500, 77], [5, 3], 4, 2, 16, 128, FP16, window, seed=3, scale=scale, q_size=size)
+
+
+def _poison_rest(cache, table, lens):
+    """Everything of the cache that no request holds: NaN codes; scales of unused pages NaN."""
+    page = cache.k.shape[2]
+    k8, v8 = cache.k.view(torch.uint8), cache.v.view(torch.uint8)
+    used = {}
+    for b, n in enumerate(lens):
+        for c in range(-(-n // page)):
+            used[table[b][c]] = min(page, n - c * page)
+    for p in range(cache.k.shape[0]):
+        n = used.get(p, 0)
+        k8[p, :, n:] = 0x7F
+        v8[p, :, :, n:] = 0xFF
+        if n == 0:
+            cache.k_scale[p] = cache.v_scale[p] = float("nan")
+
+
+def test_attention_ignores_what_no_request_holds():
+    lens, rows = [1, 16, 30, 65, 200], [1, 3, 7, 2, 40]
+    for d, page in ((128, 16), (64, 64)):
+        cache, table, start = _setup(lens, rows, 2, page, d, seed=2, extra=5)
+        q = torch.randn(start[-1], 4, d, generator=_gen(9)).to(BF16)
+        clean = ops.kv_attention(q.to(DEV), _to(cache, DEV), _i32(table), _i32(lens), _i32(start))
+        _poison_rest(cache, table, lens)
+        got = ops.kv_attention(q.to(DEV), _to(cache, DEV), _i32(table), _i32(lens), _i32(start))
+        assert torch.equal(clean, got)
+
+
+def test_attention_pages_behind_the_window_may_be_gone():
+    lens, rows, page, window = [300, 90], [4, 2], 16, 40
+    cache, table, start = _setup(lens, rows, 2, page, 64, seed=5)
+    q = torch.randn(6, 2, 64, generator=_gen(4)).to(BF16)
+    args = (_i32(lens), _i32(start))
+    want = ops.kv_attention(q.to(DEV), _to(cache, DEV), _i32(table), *args, window=window)
+    for b, (n, r) in enumerate(zip(lens, rows)):
+        for c in range((n - r - window + 1) // page):
+            table[b][c] = (-1, 1 << 30, -(1 << 31))[c % 3]
+    got = ops.kv_attention(q.to(DEV), _to(cache, DEV), _i32(table), *args, window=window)
+    assert torch.equal(want, got)
+
+
+def test_attention_missing_pages_and_poisoned_scales_give_nan():
+    """Rows that see a token without a page, of a page with a NaN scale, or of a request longer than
+    its table: NaN in every dimension.  Rows that do not, and other requests, are unharmed."""
+    lens, rows, page, d = [100, 100, 100, 40], [60, 60, 60, 3], 16, 64
+    cache, table, start = _setup(lens, rows, 2, page, d, seed=7)
+    q = torch.randn(start[-1], 4, d, generator=_gen(4)).to(FP16).to(DEV)
+    clean = ops.kv_attention(q, _to(cache, DEV), _i32(table), _i32(lens), _i32(start))
+    table[0][4] = cache.k.shape[0]               # tokens 64..79
+    cache.v_scale[table[1][5], 1] = float("nan")  # tokens 80..95 of kv head 1
+    cache.k_scale[table[2][3], 0] = float("nan")  # tokens 48..63 of kv head 0
+    dev = _to(cache, DEV)
+    got = ops.kv_attention(q, dev, _i32(table), _i32(lens), _i32(start))
+    want = torch.isnan(got)
+    bad = torch.zeros_like(want)
+    bad[64 - 40:60] = True
+    bad[60 + 80 - 40:120, 2:] = True
+    bad[120 + 48 - 40:180, :2] = True
+    assert torch.equal(want, bad)
+    assert torch.equal(got[~bad], clean[~bad])
+    short = _i32(table)[:, :6]                   # 96 tokens: requests 0 to 2 do not fit
+    got = ops.kv_attention(q, dev, short, _i32(lens), _i32(start))
+    assert torch.isnan(got[:180]).all() and torch.equal(got[180:], clean[180:])
+    got = ops.kv_attention(q, dev, _i32(table), _i32([2 ** 31 - 1] * 4), _i32(start))
+    assert torch.isnan(got).all()
+
+
+def test_attention_leaves_rows_behind_the_last_request():
+    lens, rows = [20, 33], [2, 1]
+    cache, table, start = _setup(lens, rows, 2, 16, 64, seed=1)
+    q = torch.randn(7, 4, 64, generator=_gen(4)).to(BF16).to(DEV)
+    q[3:] = float("nan")
+    out = torch.full_like(q, 5.0)
+    r = ops.kv_attention(q, _to(cache, DEV), _i32(table), _i32(lens), _i32(start), out=out)
+    assert r is out and (out[3:] == 5).all() and torch.isfinite(out[:3]).all()
+    # padded requests of a batch: no tokens, no rows
+    pad = ops.kv_attention(q, _to(cache, DEV), _i32(table + [[-1] * len(table[0])] * 3), _i32(lens + [0, 0, 0]),
+                           _i32(start + [3, 3, 3]))
+    assert torch.equal(pad[:3], out[:3])
+    # q_start that runs past the rows, or backwards: nothing outside them is touched
+    for s in ([0, 2, 90], [0, 5, 2], [-4, 1, 3], [6, 7, 2 ** 31 - 1]):
+        out.fill_(5.0)
+        ops.kv_attention(q[:5], _to(cache, DEV), _i32(table), _i32(lens), _i32(s), out=out[:5])
+        assert (out[5:] == 5).all()
+
+
+def test_attention_strided_rows_and_outputs():
+    lens = [50, 20, 64]
+    cache, table, start = _setup(lens, [1] * 3, 2, 16, 128, seed=3)
+    dev = _to(cache, DEV)
+    wide = torch.randn(3, 8 * 128 + 8, generator=_gen(4)).to(BF16).to(DEV)
+    q = wide[:, 4 * 128:8 * 128].unflatten(1, (4, 128))
+    want = ops.kv_attention(q.contiguous(), dev, _i32(table), _i32(lens))
+    assert torch.equal(want, ops.kv_attention(q, dev, _i32(table), _i32(lens)))
+    odd = torch.empty(3 * 4 * 128 + 1, dtype=BF16, device=DEV)[1:].view(3, 4, 128)
+    odd.copy_(q)
+    assert torch.equal(want, ops.kv_attention(odd, dev, _i32(table), _i32(lens)))
+    out = torch.zeros(4, 3, 136, dtype=BF16, device=DEV)
+    view = out.transpose(0, 1)[..., :128]
+    ops.kv_attention(q, dev, _i32(table), _i32(lens), out=view)
+    assert torch.equal(view, want) and (out[..., 128:] == 0).all()
+    big = torch.full((3, 90), -1, dtype=torch.int32, device=DEV)
+    big[:, :len(table[0])] = _i32(table)
+    assert torch.equal(want, ops.kv_attention(q, dev, big[:, :len(table[0])], _i32(lens)))
+
+
+def test_cache_offsets_past_32_bits():
+    """Pages more than 4 GiB into the pool, for the writer and the reader."""
+    hk, page, d = 8, 256, 512
+    pages = (5 << 30) // (hk * page * d)
+    cache = ops.kv_cache(pages, hk, page, d, DEV)
+    t = 300
+    at = [pages - 1, 3]
+    slots = torch.tensor([at[i // page] * page + i % page for i in range(t)], device=DEV)
+    k = torch.randn(t, hk, d, generator=_gen(1)).to(BF16).to(DEV)
+    v = torch.randn(t, hk, d, generator=_gen(2)).to(BF16).to(DEV)
+    small = ops.kv_cache(2, hk, page, d, DEV)
+    ops.kv_append(k, v, slots, cache)
+    ops.kv_append(k, v, torch.arange(t, device=DEV), small)
+    for x, y in zip(cache, small):
+        x, y = (z.view(torch.uint8) if z.dtype == O.E4M3 else z for z in (x, y))
+        assert torch.equal(x[at], y)
+        assert not x[at[1] + 1:pages - 1].any()
+    q = torch.randn(1, 16, d, generator=_gen(3)).to(BF16).to(DEV)
+    a = ops.kv_attention(q, cache, _i32([at]), _i32([t]))
+    assert torch.equal(a, ops.kv_attention(q, small, _i32([[0, 1]]), _i32([t])))
+
+
+def test_attention_is_deterministic_and_runs_on_any_stream():
+    lens = [3000, 40]
+    cache, table, start = _setup(lens, [1, 1], 2, 16, 128, seed=11)
+    dev = _to(cache, DEV)
+    q = torch.randn(2, 8, 128, generator=_gen(4)).to(BF16).to(DEV)
+    t, n = _i32(table), _i32(lens)
+    want = ops.kv_attention(q, dev, t, n)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for s in streams:  # two calls under way at once, each with its own scratch
+            with torch.cuda.stream(s):
+                got.append(ops.kv_attention(q, dev, t, n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, x) for x in got)
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+def test_steps_of_a_layer_in_two_graphs():
+    """Slots, projections, rope, append and attention of a padded batch over steps, captured once
+    for prompts and once for decoding (the two share the stream and the memory pool) and replayed
+    with other lengths, against the same calls made eagerly and against the oracle."""
+    hq, hk, d, page, h, b, cols = 4, 2, 64, 16, 128, 5, 12
+    g = _gen(21)
+    w = [tuple(x.to(DEV) for x in synth.linear_weights(h, n * d, 64, seed=n)) for n in (hq, hk, hk + 1)]
+    w[2] = tuple(x[:, :hk * d].contiguous() for x in w[2])
+    freq, _ = ops.rope_frequencies(d // 2, device=DEV)
+
+    def step(st, rows):
+        r = ops.kv_slots(st["ctx"], st["new"], st["table"], st["free"], st["used"], page, rows)
+        q, k, v = (y.view(rows, -1, d) for y in ops.w4a16_linear_multi(st["x"][:rows], w, 64))
+        q, k = ops.rope_rows(q, k, r.positions, freq, interleaved=True)
+        ops.kv_append(k, v, r.slots, st["cache"])
+        o = ops.kv_attention(q, st["cache"], st["table"], r.seq_lens, r.q_start, out=st["out"][:rows])
+        st["ctx"].copy_(r.seq_lens)
+        st["used"].copy_(r.status)
+        return q, k, v, r, o
+
+    def fresh():
+        return {"ctx": _i32([0] * b), "new": _i32([0] * b), "free": torch.randperm(60, generator=_gen(1)).int().to(DEV),
+                "table": torch.full((b, cols), -1, dtype=torch.int32, device=DEV), "used": _i32([0, 0, 0]),
+                "cache": ops.kv_cache(60, hk, page, d, DEV), "x": torch.zeros(70, h, dtype=BF16, device=DEV),
+                "out": torch.zeros(70, hq, d, dtype=BF16, device=DEV)}
+
+    def reset(st, other):
+        for n, x in st.items():
+            for u, y in zip(x if n == "cache" else [x], other[n] if n == "cache" else [other[n]]):
+                u.view(torch.uint8).copy_(y.view(torch.uint8))
+
+    plan = [([33, 0, 17, 1, 9], 70), ([1, 0, 1, 1, 1], 8), ([1, 0, 1, 1, 1], 8), ([0, 40, 0, 2, 0], 70),
+            ([1, 1, 1, 1, 0], 8), ([1, 1, 0, 1, 1], 8)]
+    xs = [synth.activations(70, h, seed=i).to(DEV) for i in range(len(plan))]
+    eager, replay = fresh(), fresh()
+    graphs, side = {}, torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for rows in (70, 8):
+            step(replay, rows)  # sets up what the linears keep between calls
+    torch.cuda.synchronize()
+    for rows in (70, 8):
+        graphs[rows] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graphs[rows], stream=side):
+            step(replay, rows)
+    reset(replay, eager)
+    for i, (new, rows) in enumerate(plan):
+        for st in (eager, replay):
+            st["new"].copy_(_i32(new))
+            st["x"].copy_(xs[i])
+        before = _to(eager["cache"], "cpu")
+        q, k, v, r, o = step(eager, rows)
+        graphs[rows].replay()
+        torch.cuda.synchronize()
+        n = sum(new)
+        for name in ("ctx", "table", "used"):
+            assert torch.equal(eager[name], replay[name]), (i, name)
+        _same_cache(replay["cache"], _to(eager["cache"], "cpu"))
+        assert torch.equal(eager["out"][:n], replay["out"][:n]), i
+        want = O.append(k.cpu(), v.cpu(), r.slots.tolist(), before)
+        _same_cache(eager["cache"], want)
+        ref, weighted, size = O.attention(q.cpu()[:n], want, eager["table"].tolist(), r.seq_lens.tolist(),
+                                          r.q_start.tolist(), d ** -0.5)
+        _check_out(o[:n], ref, weighted, size, d, 64)
+
+
+# ---------------------------------------------------------------------------
+# refusals of the torch-facing calls
+# ---------------------------------------------------------------------------
+def test_refusals():
+    cache = ops.kv_cache(4, 2, 16, 64, DEV)
+    x = torch.zeros(3, 2, 64, dtype=BF16, device=DEV)
+    s = torch.zeros(3, dtype=torch.int64, device=DEV)
+    q = torch.zeros(3, 4, 64, dtype=BF16, device=DEV)
+    t, n = _i32([[0, 1]] * 3), _i32([1, 2, 3])
+    for kw in (dict(page_size=24), dict(head_dim=96), dict(num_pages=0)):
+        with pytest.raises(ValueError):
+            ops.kv_cache(**{**dict(num_pages=4, kv_heads=2, page_size=16, head_dim=64, device=DEV), **kw})
+    bad = [
+        (ValueError, lambda: ops.kv_append(x[:, :1], x[:, :1], s, cache)),
+        (ValueError, lambda: ops.kv_append(x, x[:2], s, cache)),
+        (ValueError, lambda: ops.kv_append(x, x, s[:2], cache)),
+        (TypeError, lambda: ops.kv_append(x, x, s.int(), cache)),
+        (TypeError, lambda: ops.kv_append(x, x.float(), s, cache)),
+        (TypeError, lambda: ops.kv_append(x.cpu(), x, s, cache)),
+        (ValueError, lambda: ops.kv_append(x.transpose(1, 2).contiguous().transpose(1, 2), x, s, cache)),
+        (ValueError, lambda: ops.kv_append(x, x, s, cache._replace(v=cache.k))),
+        (TypeError, lambda: ops.kv_append(x, x, s, cache._replace(k=cache.k.view(torch.uint8)))),
+        (ValueError, lambda: ops.kv_append(x, x, s, cache._replace(k_scale=cache.k_scale[:3]))),
+        (TypeError, lambda: ops.kv_attention(q.float(), cache, t, n)),
+        (ValueError, lambda: ops.kv_attention(q[:, :3], cache, t, n)),
+        (ValueError, lambda: ops.kv_attention(q, cache, t[:2], n)),
+        (ValueError, lambda: ops.kv_attention(q[:2], cache, t, n)),
+        (ValueError, lambda: ops.kv_attention(q, cache, t, n, _i32([0, 3]))),
+        (TypeError, lambda: ops.kv_attention(q, cache, t, n.long())),
+        (TypeError, lambda: ops.kv_attention(q, cache, t.long(), n)),
+        (ValueError, lambda: ops.kv_attention(q, cache, t, n, window=-1)),
+        (ValueError, lambda: ops.kv_attention(q, cache, t, n, out=q)),
+        (ValueError, lambda: ops.kv_attention(q, cache, t, n, out=torch.zeros(3, 4, 65, dtype=BF16, device=DEV)[..., :64])),
+        (ValueError, lambda: ops.kv_attention(q, cache, t[:1].expand(3, 2), n)),
+        (TypeError, lambda: ops.rope_rows(q, x, s.int(), ops.rope_frequencies(64, device=DEV)[0])),
+        (TypeError, lambda: ops.rope_rows(q, x, s, ops.rope_frequencies(64, device=DEV)[0].float())),
+        (ValueError, lambda: ops.rope_rows(q, x, s, ops.rope_frequencies(66, device=DEV)[0])),
+        (ValueError, lambda: ops.rope_rows(q, x[:2], s, ops.rope_frequencies(64, device=DEV)[0])),
+        (ValueError, lambda: ops.rope_rows(q[:, :1].expand(3, 4, 64), None, s, ops.rope_frequencies(64, device=DEV)[0],
+                                           inplace=True)),
+        (ValueError, lambda: ops.rope_frequencies(7)),
+        (ValueError, lambda: ops.rope_frequencies(8, scaling="other")),
+        (ValueError, lambda: ops.kv_slots(n, n[:2], t, n, n, 16, 5)),
+        (ValueError, lambda: ops.kv_slots(n, n, t, n, n, 20, 5)),
+        (TypeError, lambda: ops.kv_slots(n.long(), n, t, n, n, 16, 5)),
+        (ValueError, lambda: ops.kv_slots(n, n, t, n, n, 16, -1)),
+        (L.GIError, lambda: ops.kv_slots(_i32([0] * 9000), _i32([0] * 9000), _i32([[0]] * 9000), n, n, 16, 5)),
+    ]
+    for i, (error, call) in enumerate(bad):
+        with pytest.raises(error):
+            call()
+            print("no refusal of call", i)
