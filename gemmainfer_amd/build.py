@@ -43,6 +43,12 @@ COMMON_FLAGS = [
     "-mllvm", "-disable-promote-alloca-to-lds",
 ]
 
+# Flags of single files.  The attention kernels hold up to 256 accumulator
+# registers a lane beside the softmax's operands: with MFMAs that read and
+# write vector registers directly the compiler moves values to accumulation registers
+# only where it runs out (spills of the 64-column kernel: 407 -> 4).
+FILE_FLAGS = {"kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def lib_path(timeline: bool = False) -> Path:
     return LIBDIR / (TIMELINE_LIBNAME if timeline else LIBNAME)
@@ -51,7 +57,7 @@ def lib_path(timeline: bool = False) -> Path:
 def _compile(src: Path, timeline: bool = False) -> Path:
     objdir = OBJDIR.with_name(OBJDIR.name + "_timeline") if timeline else OBJDIR
     obj = objdir / (src.stem + ".o")
-    cmd = [HIPCC, *COMMON_FLAGS, *(["-DGI_TIMELINE"] if timeline else []), "-c", str(src), "-o", str(obj)]
+    cmd = [HIPCC, *COMMON_FLAGS, *FILE_FLAGS.get(src.name, []), *(["-DGI_TIMELINE"] if timeline else []), "-c", str(src), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     out = "\n".join(l for l in (res.stdout + res.stderr).splitlines()
                     if "packed-fp32-ops" not in l)

@@ -140,6 +140,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int want, bool by_t
       it.first_item = first_item + it.tile * per;
       // the last tiles of a prompt see the most: they go first
       it.tile = it.tiles - 1 - it.tile;
+      for (int* f : {&it.b, &it.tile, &it.tiles, &it.chunk_no, &it.chunk, &it.q0, &it.rows, &it.len, &it.first_item})
+        *f = __builtin_amdgcn_readfirstlane(*f);
       return true;
     }
     items = __shfl(item_end, kWave - 1, kWave);
@@ -209,10 +211,30 @@ struct Qk<true> {
 // ---------------------------------------------------------------------------
 // the kernel
 // ---------------------------------------------------------------------------
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// max over the four lanes of a column (lane % 16), to all of them
+__device__ __forceinline__ float column_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// What a wave reads of one unit.
+struct UnitRef {
+  const uint8_t* k;
+  const uint8_t* v;
+  float ks, vs;
+};
+
 // The four waves of a workgroup take turns at units of 64 cache rows; each has
 // its own running softmax over 16 * CT columns, joined at the end through LDS.
-// No barrier and no LDS in the loop: lane (i = lane % 16, g = lane / 16) reads
-// from the cache just what its place in the MFMA operands needs.
+// No barrier in the loop, and K and V do not pass through LDS: lane (i = lane %
+// 16, g = lane / 16) reads from the cache just what its place in the MFMA
+// operands needs.
 //   S^T = K Q^T, 16x16x32: operand A's row i of product j is cache row 16 (i / 4) +
 //     4 j + i % 4 of the unit, so that the four results of lane (i, g) are rows
 //     16 g + 4 j ... + 3 of column i: after j = 0..3 a lane holds the 16
@@ -223,27 +245,39 @@ struct Qk<true> {
 // So neither the scores nor V cross lanes, and a lane needs one K and one V
 // scale per unit.  A column's maximum is the only exchange (two lane swaps).
 //
+// A unit is eight steps of D / 64 loads a lane: four K tiles, then V in four
+// parts.  The loads of the next kRing - 1 steps are always in flight, over the
+// end of a unit as well, so the matrix cores and the softmax run while HBM (or
+// L2) delivers.
+//
 // V's scale joins the exponent: t = s + log2(vs), weights 2^(t - m), m over t.
 // The sum of softmax weights is then sum 2^(t - m) / vs.  With it the weights
 // of V's codes never exceed 2^(kBias + kSlack) whatever the scales are, and the
-// maximum is over what each row can contribute.
+// maximum is over what each row can contribute.  m follows the true maximum
+// only when it is kSlack behind: the sums are scaled anew a few times a call,
+// not once a unit.
 template <int D, int CT, bool F16>
-__global__ __launch_bounds__(kThreads, 1) void kv_attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kThreads, D * CT <= 256 ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
   constexpr int RT = 16 * CT;
-  constexpr int KS = D / 64;   // 16-byte K loads of a lane per row
+  constexpr int KS = D / 64;   // 16-byte loads of a lane per step
   constexpr int DT = D / 16;   // dimension tiles of the output
+  constexpr int kRing = D <= 128 ? 8 : 4;
   constexpr bool kQLds = CT * D > 512;
+  constexpr int kPitch = D + 4;
+  constexpr int kBufs = RT * kPitch * 16 <= 140000 ? 4 : 1;  // waves that hand over their sums at once
+  constexpr size_t kRedBytes = (size_t)kBufs * RT * kPitch * 4, kQBytes = kQLds ? (size_t)CT * 2 * KS * kWave * 16 : 16;
   typedef typename Qk<F16>::frag frag;
-  __shared__ float red[RT][D + 4];
+  __shared__ __align__(16) char lds[kRedBytes > kQBytes ? kRedBytes : kQBytes];
   __shared__ float red_m[kWaves][RT], red_l[kWaves][RT];
-  __shared__ uint4 q_lds[kQLds ? CT * 2 * KS * kWave : 1];
+  uint4* q_lds = (uint4*)lds;
+  float* red = (float*)lds;
 
   const int hk = blockIdx.x % a.Hk;
   Item it;
   if (!find_item<RT>(a, blockIdx.x / a.Hk, false, it)) return;
   const Span sp = span_of<RT>(a, it);
   if (it.chunk_no >= sp.chunks) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int i16 = lane & 15, g = lane >> 4;
   const int page_mask = (1 << a.log_page) - 1;
   const int r0 = it.tile * RT;
@@ -280,112 +314,161 @@ __global__ __launch_bounds__(kThreads, 1) void kv_attention_kernel(AttnArgs a) {
   }
 
   const int32_t* table = a.table + it.b * a.table_stride;
-  auto page_of = [&](int tok) -> int64_t {
-    const int col = tok >> a.log_page;
-    return col < a.cols ? (int64_t)table[col] : (int64_t)-1;
-  };
-  const int u_end = min(sp.lo + (it.chunk_no + 1) * it.chunk, sp.hi);
-  const int u_first = sp.lo + it.chunk_no * it.chunk + wave;
   const int grp_k = 16 * (i16 >> 2);
-  for (int u = u_first; u < u_end; u += kWaves) {
+  auto page_of = [&](int tok) -> int {
+    const int col = tok >> a.log_page;
+    return col < a.cols ? table[col] : -1;
+  };
+  auto ref_of = [&](int u, int kp, int vp) -> UnitRef {
     const int tok = u * kUnit;
-    int64_t kp = page_of(tok + grp_k), vp = page_of(tok + 16 * g);
     // a page that is not there: nothing is read from where it points, and its
     // rows, if they are seen at all, have no scale
-    if (kp < 0 || kp >= a.num_pages) kp = 0;
-    const bool bad = vp < 0 || vp >= a.num_pages || it.over;
-    if (vp < 0 || vp >= a.num_pages) vp = 0;
-    const uint8_t* kb = a.kc + (((kp * a.Hk + hk) << a.log_page) + ((tok + grp_k) & page_mask) + (i16 & 3)) * D + 16 * g;
-    const uint8_t* vb = a.vc + (((vp * a.Hk + hk) * D + i16) << a.log_page) + ((tok + 16 * g) & page_mask);
-    float ks = a.ks[vp * a.Hk + hk], vs = a.vs[vp * a.Hk + hk];
-    if (bad) ks = vs = __uint_as_float(0x7fc00000u);
+    const int64_t kq = kp < 0 || kp >= a.num_pages ? 0 : kp;
+    const bool bad = vp < 0 || vp >= a.num_pages;
+    const int64_t vq = bad ? 0 : vp;
+    UnitRef r;
+    r.k = a.kc + (((kq * a.Hk + hk) << a.log_page) + ((tok + grp_k) & page_mask) + (i16 & 3)) * D + 16 * g;
+    r.v = a.vc + (((vq * a.Hk + hk) * D + i16) << a.log_page) + ((tok + 16 * g) & page_mask);
+    r.ks = a.ks[vq * a.Hk + hk];
+    r.vs = a.vs[vq * a.Hk + hk];
+    if (bad || it.over) r.ks = r.vs = __uint_as_float(0x7fc00000u);
+    return r;
+  };
+  const int u_end = uniform(min(sp.lo + (it.chunk_no + 1) * it.chunk, sp.hi));
+  const int u_first = uniform(sp.lo + it.chunk_no * it.chunk + wave);
+  const int pos_min = uniform(sp.pos_min), pos_max = uniform(sp.pos_max);
 
-    // ---- scores
-    f32x4_t s[CT][4];
+  if (u_first < u_end) {
+    const int u_last = u_first + (u_end - 1 - u_first) / kWaves * kWaves;
+    uint4 ring[kRing][KS];
+    // loads step `st` of a unit into its place of the ring
+    auto issue = [&](const UnitRef& r, int st) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+      for (int i = 0; i < KS; ++i)
+        ring[st % kRing][i] = st < 4 ? *(const uint4*)(r.k + st * 4 * D + i * 64)
+                                     : *(const uint4*)(r.v + ((size_t)(((st - 4) * KS + i) * 16) << a.log_page));
+    };
+    UnitRef cur = ref_of(u_first, page_of(u_first * kUnit + grp_k), page_of(u_first * kUnit + 16 * g));
+    const int u1 = min(u_first + kWaves, u_last);
+    UnitRef nxt = ref_of(u1, page_of(u1 * kUnit + grp_k), page_of(u1 * kUnit + 16 * g));
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) s[ct][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int st = 0; st < KS; ++st) {
-        const uint4 w = *(const uint4*)(kb + j * 4 * D + st * 64);
-        const frag k0 = Qk<F16>::codes(w.x, w.y), k1 = Qk<F16>::codes(w.z, w.w);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const frag q0 = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * st) * kWave + lane])
-                                : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * st];
-          const frag q1 = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * st + 1) * kWave + lane])
-                                : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * st + 1];
-          s[ct][j] = Qk<F16>::mfma(k0, q0, s[ct][j]);
-          s[ct][j] = Qk<F16>::mfma(k1, q1, s[ct][j]);
-        }
-      }
-    }
+    for (int st = 0; st < kRing - 1; ++st) issue(cur, st);
 
-    // ---- weights
-    const float cs = ks * a.scale, cv = __log2f(vs), inv_vs = 1.f / vs;
-    const bool edge = tok + kUnit - 1 > sp.pos_min || (a.window > 0 && tok <= sp.pos_max - a.window);
-    f16x8_t p[CT][2];
+    for (int u = u_first; u < u_end; u += kWaves) {
+      const int tok = u * kUnit;
+      // past the last unit the loads repeat it (they are not used)
+      const int u2 = min(u + 2 * kWaves, u_last);
+      const int kp2 = page_of(u2 * kUnit + grp_k), vp2 = page_of(u2 * kUnit + 16 * g);
+      const bool edge = tok + kUnit - 1 > pos_min || (a.window > 0 && tok <= pos_max - a.window);
+      f32x4_t s[CT][4];
+      f16x8_t p[CT][2];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float top = -INFINITY;
+      for (int st = 0; st < 8; ++st) {
+        if (st + kRing - 1 < 8) issue(cur, st + kRing - 1);
+        else issue(nxt, st + kRing - 1 - 8);
+        __builtin_amdgcn_sched_barrier(0);
+        if (st < 4) {
+          // ---- scores of four rows of each group
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+          for (int ct = 0; ct < CT; ++ct) s[ct][st] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float t = fmaf(s[ct][j][r], cs, cv);
-          if (edge) {
-            const int x = tok + 16 * g + 4 * j + r;
-            const bool seen = x <= hi_pos[ct] && (a.window <= 0 || x > hi_pos[ct] - a.window);
-            t = seen ? t : -INFINITY;
+          for (int i = 0; i < KS; ++i) {
+            const uint4 w = ring[st % kRing][i];
+            const frag k0 = Qk<F16>::codes(w.x, w.y), k1 = Qk<F16>::codes(w.z, w.w);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const frag q0 = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * i) * kWave + lane])
+                                    : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * i];
+              s[ct][st] = Qk<F16>::mfma(k0, q0, s[ct][st]);
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const frag q1 = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * i + 1) * kWave + lane])
+                                    : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * i + 1];
+              s[ct][st] = Qk<F16>::mfma(k1, q1, s[ct][st]);
+            }
           }
-          s[ct][j][r] = t;
-          top = fmaxf(top, t);
         }
-      top = fmaxf(top, __shfl_xor(top, 16, kWave));
-      top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      if (__any(top > m[ct] + kSlack)) {
-        const float now = fmaxf(m[ct], top);
-        const float next = now == -INFINITY ? 0.f : now;
-        const float f = m[ct] == -INFINITY ? 0.f : exp2f(mref[ct] - next);  // -inf: nothing was added yet
-        m[ct] = now;
-        mref[ct] = next;
-        l[ct] *= f;
+        if (st == 3) {
+          // ---- weights
+          const float cs = cur.ks * a.scale, cv = __log2f(cur.vs), inv_vs = 1.f / cur.vs;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[ct][dt] *= f;
-      }
-      float sum = 0.f;
+          for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float w = exp2f(s[ct][j][r] - mref[ct] + kBias);
-          sum += w;
-          p[ct][j >> 1][(j & 1) * 4 + r] = (_Float16)w;
+              for (int r = 0; r < 4; ++r) s[ct][j][r] = fmaf(s[ct][j][r], cs, cv);
+            if (edge) {
+              const int hi = hi_pos[ct] - (tok + 16 * g), lo = a.window > 0 ? hi - a.window : -1;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  s[ct][j][r] = 4 * j + r <= hi && 4 * j + r > lo ? s[ct][j][r] : -INFINITY;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) top = fmaxf(top, s[ct][j][r]);
+            top = column_max(top);
+            if (__any(top > m[ct] + kSlack)) {
+              const float now = fmaxf(m[ct], top);
+              const float next = now == -INFINITY ? 0.f : now;
+              const float f = m[ct] == -INFINITY ? 0.f : exp2_fast(mref[ct] - next);  // -inf: nothing was added yet
+              m[ct] = now;
+              mref[ct] = next;
+              l[ct] *= f;
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt) acc[ct][dt] *= f;
+            }
+            const float shift = kBias - mref[ct];
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float w = exp2_fast(s[ct][j][r] + shift);
+                sum += w;
+                p[ct][j >> 1][(j & 1) * 4 + r] = (_Float16)w;
+              }
+            // rows that are not seen weigh nothing, whatever their page's scale is
+            l[ct] += sum == 0.f ? 0.f : sum * inv_vs;
+          }
+        }
+        if (st >= 4) {
+          // ---- O^T += V^T P^T, a quarter of the dimensions
+          if (edge) {  // rows that no column sees may hold anything
+            const int last = min(pos_max - (tok + 16 * g), 15);
+            const int first = a.window > 0 ? pos_min - a.window + 1 - (tok + 16 * g) : 0;
+            uint32_t keep[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              keep[x] = 0;
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                if (4 * x + y <= last && 4 * x + y >= first) keep[x] |= 0xffu << (8 * y);
+            }
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+              uint4& w = ring[st % kRing][i];
+              w = make_uint4(w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            const uint4 w = ring[st % kRing][i];
+            const f16x8_t v0 = codes_f16(w.x, w.y), v1 = codes_f16(w.z, w.w);
+            const int dt = (st - 4) * KS + i;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) acc[ct][dt] = mfma_f16(v0, p[ct][0], acc[ct][dt]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) acc[ct][dt] = mfma_f16(v1, p[ct][1], acc[ct][dt]);
+          }
         }
       }
-      // rows that are not seen weigh nothing, whatever their page's scale is
-      l[ct] += sum == 0.f ? 0.f : sum * inv_vs;
-    }
-
-    // ---- O^T += V^T P^T
-    const int last = min(sp.pos_max - (tok + 16 * g), 15), firstx = a.window > 0 ? sp.pos_min - a.window + 1 - (tok + 16 * g) : 0;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      uint4 w = *(const uint4*)(vb + ((dt * 16) << a.log_page));
-      if (edge) {  // rows that no column sees may hold anything
-        uint32_t o[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int x = 0; x < 16; ++x)
-          if (x > last || x < firstx) o[x >> 2] &= ~(0xffu << (8 * (x & 3)));
-        w = make_uint4(o[0], o[1], o[2], o[3]);
-      }
-      const f16x8_t v0 = codes_f16(w.x, w.y), v1 = codes_f16(w.z, w.w);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        acc[ct][dt] = mfma_f16(v0, p[ct][0], acc[ct][dt]);
-        acc[ct][dt] = mfma_f16(v1, p[ct][1], acc[ct][dt]);
-      }
+      cur = nxt;
+      nxt = ref_of(u2, kp2, vp2);
     }
   }
 
@@ -406,17 +489,20 @@ __global__ __launch_bounds__(kThreads, 1) void kv_attention_kernel(AttnArgs a) {
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red_m[w][ct * 16 + i16]);
-    f[ct] = m[ct] == -INFINITY ? 0.f : exp2f(mref[ct] - top);
+    f[ct] = m[ct] == -INFINITY ? 0.f : exp2_fast(mref[ct] - top);
+    if (m[ct] == -INFINITY && l[ct] != l[ct]) f[ct] = l[ct];  // only scores without a value: they stay NaN
   }
-  for (int w = 0; w < kWaves; ++w) {
-    if (w == wave) {
+#pragma unroll
+  for (int w = 0; w < kWaves / kBufs; ++w) {
+    if (kBufs == kWaves || w == wave) {
+      float* buf = red + (kBufs == kWaves ? wave * RT * kPitch : 0);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          f32x4_t* dst = (f32x4_t*)&red[ct * 16 + i16][dt * 16 + 4 * g];
+          f32x4_t* dst = (f32x4_t*)(buf + (ct * 16 + i16) * kPitch + dt * 16 + 4 * g);
           const f32x4_t v = acc[ct][dt] * f[ct];
-          *dst = w == 0 ? v : *dst + v;
+          *dst = kBufs == kWaves || w == 0 ? v : *dst + v;
         }
     }
     __syncthreads();
@@ -428,19 +514,28 @@ __global__ __launch_bounds__(kThreads, 1) void kv_attention_kernel(AttnArgs a) {
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red_m[w][c]);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
-      if (red_m[w][c] != -INFINITY) sum += red_l[w][c] * exp2f(red_m[w][c] - top);
+      if (red_m[w][c] != -INFINITY) sum += red_l[w][c] * exp2_fast(red_m[w][c] - top);
+    f32x4_t o0 = {0.f, 0.f, 0.f, 0.f}, o1 = o0;
+#pragma unroll
+    for (int w = 0; w < kBufs; ++w) {
+      o0 += *(const f32x4_t*)(red + (w * RT + c) * kPitch + d);
+      o1 += *(const f32x4_t*)(red + (w * RT + c) * kPitch + d + 4);
+    }
     if (sp.chunks == 1) {
       const int r = r0 + c, row = r / a.G, head = hk * a.G + (r - row * a.G);
       uint16_t o[8];
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) o[x] = Qk<F16>::out(red[c][d + x] * inv);
+      for (int x = 0; x < 4; ++x) {
+        o[x] = Qk<F16>::out(o0[x] * inv);
+        o[4 + x] = Qk<F16>::out(o1[x] * inv);
+      }
       *(uint4*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
           make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
     } else {
       float* dst = a.part + ((size_t)blockIdx.x * RT + c) * D + d;
-      *(float4*)dst = make_float4(red[c][d], red[c][d + 1], red[c][d + 2], red[c][d + 3]);
-      *(float4*)(dst + 4) = make_float4(red[c][d + 4], red[c][d + 5], red[c][d + 6], red[c][d + 7]);
+      *(f32x4_t*)dst = o0;
+      *(f32x4_t*)(dst + 4) = o1;
       if (d == 0) {
         float* ml = a.part + (size_t)a.max_items * a.Hk * RT * D + ((size_t)blockIdx.x * RT + c) * 2;
         ml[0] = top;
