@@ -95,10 +95,11 @@ __global__ __launch_bounds__(256) void rope_kernel(T* q, T* k, const T* cs, cons
 // p becomes (x1 c - x2 s, x2 c + x1 s), c = m cos(p f), s = m sin(p f).  The
 // angle is formed in fp64 and reduced to (-1/2, 1/2] turns before it is rounded
 // to fp32: at a position of 10^6 an fp32 product would be off by up to 0.03
-// radians, a reduced one by 1e-7.  One workgroup a row: its cos and sin are
-// worked out once, into LDS, and serve every head of q and k.  Bound by HBM:
-// each element is read and written once.
-constexpr int kRopeThreads = 256;
+// radians, a reduced one by 1e-7.  A thread takes one unit (16 bytes, or a pair,
+// of each half) of one head of one row; a workgroup the units of one row, whose cos and
+// sin its threads work out once, into LDS, while their elements are on the way.  Bound by HBM: each
+// element is read and written once.
+constexpr int kRopeThreads = 1024;  // at most
 constexpr int kRopeMaxPairs = 512;
 
 struct RopeArgs {
@@ -109,6 +110,7 @@ struct RopeArgs {
   const double* freq;
   float mscale;
   int heads[2], D, pairs;
+  int turn, units;     // units of a head that turn, and with those that are only copied
 };
 
 // Explicit fused steps, each rounded to fp32 (for fp16 results the compiler
@@ -120,87 +122,66 @@ __device__ __forceinline__ void turn_pair(float x1, float x2, float c, float s, 
   asm("" : "+v"(y1), "+v"(y2));
 }
 
-template <typename T>
-struct alignas(16) Pack8 {
-  T v[8];
+template <typename T, int N>
+struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
+  T v[N];
 };
 
-// kVec: 8 elements of a head at a time (rows, heads and the halves 16-byte
-// aligned); otherwise one pair at a time.
+// kVec: units of 8 elements (rows, heads and the halves 16-byte aligned), 8
+// pairs where the halves are apart and 4 where pairs are adjacent; otherwise a
+// unit is a pair, or one element that is copied.
 template <typename T, bool kInter, bool kVec>
 __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs a) {
+  constexpr int N = kVec ? 8 : 1;
   __shared__ float cs[kRopeMaxPairs], sn[kRopeMaxPairs];
   const int64_t row = blockIdx.x;
+  const int R = 2 * a.pairs;
+  const int i = blockIdx.y * blockDim.x + threadIdx.x;
+  const int h = i / a.units, u = i - h * a.units;
+  const bool on = h < a.heads[0] + a.heads[1], turns = u < a.turn;
+  const int w = h < a.heads[0] ? 0 : 1, hw = h - (w ? a.heads[0] : 0);
+  // the unit's elements: [d1, d1 + N) and, of a unit that turns and has its second half apart, [d2, d2 + N)
+  const bool two = turns && (!kInter || !kVec);
+  const int d1 = turns ? (kInter && !kVec ? 2 * u : u * N) : R + (u - a.turn) * N;
+  const int d2 = kInter ? d1 + 1 : a.pairs + u * N;
+  Pack<T, N> v1, v2;
+  if (on) {
+    const T* x = (const T*)a.in[w] + row * a.in_st[w] + hw * a.in_sh[w];
+    v1 = *(const Pack<T, N>*)(x + d1);
+    if (two) v2 = *(const Pack<T, N>*)(x + d2);
+  }
   const double p = (double)a.pos[row];
-  for (int i = threadIdx.x; i < a.pairs; i += kRopeThreads) {
-    const double turns = p * a.freq[i] * 0.15915494309189535;  // 1 / (2 pi)
-    const float r = (float)(turns - rint(turns));
+  for (int j = threadIdx.x; j < a.pairs; j += blockDim.x) {
+    const double t = p * a.freq[j] * 0.15915494309189535;  // 1 / (2 pi)
+    const float r = (float)(t - rint(t));
     float s, c;
     sincospif(2.f * r, &s, &c);
-    cs[i] = c * a.mscale;
-    sn[i] = s * a.mscale;
+    cs[j] = c * a.mscale;
+    sn[j] = s * a.mscale;
   }
   __syncthreads();
-  const int R = 2 * a.pairs;
+  if (!on) return;
+  T* y = (T*)a.out[w] + row * a.out_st[w] + hw * a.out_sh[w];
+  if (turns) {
+    float y1, y2;
+    if (two) {
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const T* in = (const T*)a.in[w] + row * a.in_st[w];
-    T* out = (T*)a.out[w] + row * a.out_st[w];
-    if (kVec) {
-      // units of a head: the rotated ones (8 pairs each where halves are apart,
-      // 4 where pairs are adjacent), then those behind them, only copied
-      const int turn = kInter ? R >> 3 : R >> 4, rest = (a.D - R) >> 3;
-      const int unit = turn + (in == out ? 0 : rest);
-      for (int i = threadIdx.x; i < a.heads[w] * unit; i += kRopeThreads) {
-        const int h = i / unit, u = i - h * unit;
-        const T* x = in + h * a.in_sh[w];
-        T* y = out + h * a.out_sh[w];
-        if (u >= turn) {
-          const int d = R + (u - turn) * 8;
-          *(Pack8<T>*)(y + d) = *(const Pack8<T>*)(x + d);
-        } else if (kInter) {
-          const Pack8<T> v = *(const Pack8<T>*)(x + u * 8);
-          Pack8<T> o;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float y1, y2;
-            turn_pair(ld(v.v, 2 * j), ld(v.v, 2 * j + 1), cs[u * 4 + j], sn[u * 4 + j], y1, y2);
-            st(o.v, 2 * j, y1);
-            st(o.v, 2 * j + 1, y2);
-          }
-          *(Pack8<T>*)(y + u * 8) = o;
-        } else {
-          const Pack8<T> v1 = *(const Pack8<T>*)(x + u * 8), v2 = *(const Pack8<T>*)(x + a.pairs + u * 8);
-          Pack8<T> o1, o2;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float y1, y2;
-            turn_pair(ld(v1.v, j), ld(v2.v, j), cs[u * 8 + j], sn[u * 8 + j], y1, y2);
-            st(o1.v, j, y1);
-            st(o2.v, j, y2);
-          }
-          *(Pack8<T>*)(y + u * 8) = o1;
-          *(Pack8<T>*)(y + a.pairs + u * 8) = o2;
-        }
+      for (int j = 0; j < N; ++j) {
+        turn_pair(ld(v1.v, j), ld(v2.v, j), cs[u * N + j], sn[u * N + j], y1, y2);
+        st(v1.v, j, y1);
+        st(v2.v, j, y2);
       }
+      *(Pack<T, N>*)(y + d2) = v2;
     } else {
-      const int unit = a.pairs + (in == out ? 0 : a.D - R);
-      for (int i = threadIdx.x; i < a.heads[w] * unit; i += kRopeThreads) {
-        const int h = i / unit, u = i - h * unit;
-        const T* x = in + h * a.in_sh[w];
-        T* y = out + h * a.out_sh[w];
-        if (u >= a.pairs) {
-          y[R + u - a.pairs] = x[R + u - a.pairs];
-          continue;
-        }
-        const int d1 = kInter ? 2 * u : u, d2 = kInter ? 2 * u + 1 : a.pairs + u;
-        float y1, y2;
-        turn_pair(ld(x, d1), ld(x, d2), cs[u], sn[u], y1, y2);
-        st(y, d1, y1);
-        st(y, d2, y2);
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) {
+        turn_pair(ld(v1.v, 2 * j), ld(v1.v, 2 * j + 1), cs[u * (N / 2) + j], sn[u * (N / 2) + j], y1, y2);
+        st(v1.v, 2 * j, y1);
+        st(v1.v, 2 * j + 1, y2);
       }
     }
   }
+  *(Pack<T, N>*)(y + d1) = v1;
 }
 
 int check_dtype(int dt, const char* who) {
@@ -293,7 +274,7 @@ int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, con
     return fail(GI_ERR_INVALID_ARG, "rope_rows: null pointer");
   RopeArgs a{{q, k}, {q_out, k_out}, {q_strides[0], k_strides[0]}, {q_strides[1], k_strides[1]},
              {qo_strides[0], ko_strides[0]}, {qo_strides[1], ko_strides[1]}, positions, inv_freq, mscale, {Hq, Hk}, D,
-             rotary_dim / 2};
+             rotary_dim / 2, 0, 0};
   const int size = dtype == GI_DTYPE_FP32 ? 4 : 2;
   bool vec = D % 8 == 0 && rotary_dim % (interleaved ? 8 : 16) == 0;
   for (int w = 0; w < 2; ++w) {
@@ -301,10 +282,21 @@ int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, con
     vec = vec && ((uintptr_t)a.in[w] & 15) == 0 && ((uintptr_t)a.out[w] & 15) == 0;
     for (const int64_t s : {a.in_st[w], a.in_sh[w], a.out_st[w], a.out_sh[w]}) vec = vec && s * size % 16 == 0;
   }
-#define GI_ROPE_V(T_, I_)                                                                                      \
-  do {                                                                                                         \
-    if (vec) hipLaunchKernelGGL((rope_rows_kernel<T_, I_, true>), dim3(T), dim3(kRopeThreads), 0, stream, a);  \
-    else hipLaunchKernelGGL((rope_rows_kernel<T_, I_, false>), dim3(T), dim3(kRopeThreads), 0, stream, a);     \
+  // dimensions that do not turn are left alone where the result takes the place of the input
+  const bool copy = (Hq > 0 && q != q_out) || (Hk > 0 && k != k_out);
+  a.turn = !vec ? a.pairs : interleaved ? rotary_dim / 8 : rotary_dim / 16;
+  a.units = a.turn + (copy ? (D - rotary_dim) / (vec ? 8 : 1) : 0);
+  // few rows are spread over workgroups of 256; of many, each row is one workgroup where it fits
+  // (2047 rows of 16 + 8 heads of 256: 12.6 us in workgroups of 256, which work the row's angles out twice)
+  const int64_t all = (int64_t)(Hq + Hk) * a.units;
+  const int threads = T < 256 ? 256 : (int)(all < kRopeThreads ? (all + 63) / 64 * 64 : kRopeThreads);
+  const int64_t parts = (all + threads - 1) / threads;
+  if (parts > 65535) return fail(GI_ERR_UNSUPPORTED, "rope_rows: too many heads");
+  const dim3 grid(T, (unsigned)parts);
+#define GI_ROPE_V(T_, I_)                                                                                 \
+  do {                                                                                                    \
+    if (vec) hipLaunchKernelGGL((rope_rows_kernel<T_, I_, true>), grid, dim3(threads), 0, stream, a);  \
+    else hipLaunchKernelGGL((rope_rows_kernel<T_, I_, false>), grid, dim3(threads), 0, stream, a);     \
   } while (0)
 #define GI_ROPE_I(T_)                 \
   do {                                \

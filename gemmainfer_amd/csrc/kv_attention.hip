@@ -27,6 +27,9 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kUnit = 64;      // cache rows a wave takes at a time
 constexpr int kMinChunk = 4;   // units: one a wave
+constexpr int kFree = 0x8f;
+// what a compute unit holds of a kernel: by its registers, two waves a SIMD or one
+constexpr int workgroups_per_cu(int D, int CT) { return D * CT <= 256 && CT <= 2 ? 2 : 1; }
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights go to the matrix cores in fp16 as 2^(t - m + kBias), at most 2^(kBias
 // + kSlack): fp16 is normal down to 2^-14, so a weight 2^-21 of the largest
@@ -114,7 +117,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int want, bool by_t
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, kWave);
-  const int chunk = (int)max((total + a.target - 1) / a.target, (long long)kMinChunk);
+  int chunk = (int)max((total + a.target - 1) / a.target, (long long)kMinChunk);
+  chunk = (chunk + kWaves - 1) / kWaves * kWaves;
   int items = 0, tiles = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
     const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
@@ -245,10 +249,11 @@ struct UnitRef {
 // So neither the scores nor V cross lanes, and a lane needs one K and one V
 // scale per unit.  A column's maximum is the only exchange (two lane swaps).
 //
-// A unit is eight steps of D / 64 loads a lane: four K tiles, then V in four
-// parts.  The loads of the next kRing - 1 steps are always in flight, over the
+// A unit is D / 64 steps of K and as many of V, each 64 dimensions of 64 rows in four loads a
+// lane.  The loads of the next kRing - 1 steps are always in flight, over the
 // end of a unit as well, so the matrix cores and the softmax run while HBM (or
-// L2) delivers.
+// L2) delivers.  A K step meets its two Q operands of a column tile with all
+// four products, so Q from LDS (where it does not fit in registers) is read once a unit.
 //
 // V's scale joins the exponent: t = s + log2(vs), weights 2^(t - m), m over t.
 // The sum of softmax weights is then sum 2^(t - m) / vs.  With it the weights
@@ -257,15 +262,17 @@ struct UnitRef {
 // only when it is kSlack behind: the sums are scaled anew a few times a call,
 // not once a unit.
 template <int D, int CT, bool F16>
-__global__ __launch_bounds__(kThreads, D * CT <= 256 ? 2 : 1) void kv_attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attention_kernel(AttnArgs a) {
   constexpr int RT = 16 * CT;
-  constexpr int KS = D / 64;   // 16-byte loads of a lane per step
+  constexpr int KS = D / 64;   // steps of K, and of V: 64 dimensions, four 16-byte loads of a lane
   constexpr int DT = D / 16;   // dimension tiles of the output
-  constexpr int kRing = D <= 128 ? 8 : 4;
+  constexpr int kSteps = 2 * KS;
+  constexpr int kRing = D == 64 ? 2 : D == 512 ? 8 : 4;
   constexpr bool kQLds = CT * D > 512;
-  constexpr int kPitch = D + 4;
-  constexpr int kBufs = RT * kPitch * 16 <= 140000 ? 4 : 1;  // waves that hand over their sums at once
-  constexpr size_t kRedBytes = (size_t)kBufs * RT * kPitch * 4, kQBytes = kQLds ? (size_t)CT * 2 * KS * kWave * 16 : 16;
+  // the waves' sums meet in LDS, a part of the dimensions at a time where they do not fit together
+  constexpr int kParts = (size_t)RT * (D + 4) * kWaves * 4 <= 140000 ? 1 : 2;
+  constexpr int DP = D / kParts, kPitch = DP + 4;
+  constexpr size_t kRedBytes = (size_t)kWaves * RT * kPitch * 4, kQBytes = kQLds ? (size_t)CT * 2 * KS * kWave * 16 : 16;
   typedef typename Qk<F16>::frag frag;
   __shared__ __align__(16) char lds[kRedBytes > kQBytes ? kRedBytes : kQBytes];
   __shared__ float red_m[kWaves][RT], red_l[kWaves][RT];
@@ -340,13 +347,13 @@ __global__ __launch_bounds__(kThreads, D * CT <= 256 ? 2 : 1) void kv_attention_
 
   if (u_first < u_end) {
     const int u_last = u_first + (u_end - 1 - u_first) / kWaves * kWaves;
-    uint4 ring[kRing][KS];
+    uint4 ring[kRing][4];
     // loads step `st` of a unit into its place of the ring
     auto issue = [&](const UnitRef& r, int st) {
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-        ring[st % kRing][i] = st < 4 ? *(const uint4*)(r.k + st * 4 * D + i * 64)
-                                     : *(const uint4*)(r.v + ((size_t)(((st - 4) * KS + i) * 16) << a.log_page));
+      for (int i = 0; i < 4; ++i)
+        ring[st % kRing][i] = st < KS ? *(const uint4*)(r.k + i * 4 * D + st * 64)
+                                      : *(const uint4*)(r.v + ((size_t)(((st - KS) * 4 + i) * 16) << a.log_page));
     };
     UnitRef cur = ref_of(u_first, page_of(u_first * kUnit + grp_k), page_of(u_first * kUnit + 16 * g));
     const int u1 = min(u_first + kWaves, u_last);
@@ -363,33 +370,34 @@ __global__ __launch_bounds__(kThreads, D * CT <= 256 ? 2 : 1) void kv_attention_
       f32x4_t s[CT][4];
       f16x8_t p[CT][2];
 #pragma unroll
-      for (int st = 0; st < 8; ++st) {
-        if (st + kRing - 1 < 8) issue(cur, st + kRing - 1);
-        else issue(nxt, st + kRing - 1 - 8);
-        __builtin_amdgcn_sched_barrier(0);
-        if (st < 4) {
-          // ---- scores of four rows of each group
+      for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) s[ct][st] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < 4; ++j) s[ct][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            const uint4 w = ring[st % kRing][i];
-            const frag k0 = Qk<F16>::codes(w.x, w.y), k1 = Qk<F16>::codes(w.z, w.w);
+      for (int st = 0; st < kSteps; ++st) {
+        if (st + kRing - 1 < kSteps) issue(cur, st + kRing - 1);
+        else issue(nxt, st + kRing - 1 - kSteps);
+        __builtin_amdgcn_sched_barrier(kFree);
+        if (st < KS) {
+          // ---- scores, 64 dimensions
+          frag k[4][2];
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              const frag q0 = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * i) * kWave + lane])
-                                    : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * i];
-              s[ct][st] = Qk<F16>::mfma(k0, q0, s[ct][st]);
-            }
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              const frag q1 = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * i + 1) * kWave + lane])
-                                    : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * i + 1];
-              s[ct][st] = Qk<F16>::mfma(k1, q1, s[ct][st]);
-            }
+          for (int j = 0; j < 4; ++j) {
+            const uint4 w = ring[st % kRing][j];
+            k[j][0] = Qk<F16>::codes(w.x, w.y);
+            k[j][1] = Qk<F16>::codes(w.z, w.w);
           }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const frag q = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * st + h) * kWave + lane])
+                                   : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * st + h];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s[ct][j] = Qk<F16>::mfma(k[j][h], q, s[ct][j]);
+            }
         }
-        if (st == 3) {
+        if (st == KS - 1) {
           // ---- weights
           const float cs = cur.ks * a.scale, cv = __log2f(cur.vs), inv_vs = 1.f / cur.vs;
 #pragma unroll
@@ -436,8 +444,8 @@ __global__ __launch_bounds__(kThreads, D * CT <= 256 ? 2 : 1) void kv_attention_
             l[ct] += sum == 0.f ? 0.f : sum * inv_vs;
           }
         }
-        if (st >= 4) {
-          // ---- O^T += V^T P^T, a quarter of the dimensions
+        if (st >= KS) {
+          // ---- O^T += V^T P^T, 64 dimensions
           if (edge) {  // rows that no column sees may hold anything
             const int last = min(pos_max - (tok + 16 * g), 15);
             const int first = a.window > 0 ? pos_min - a.window + 1 - (tok + 16 * g) : 0;
@@ -450,16 +458,16 @@ __global__ __launch_bounds__(kThreads, D * CT <= 256 ? 2 : 1) void kv_attention_
                 if (4 * x + y <= last && 4 * x + y >= first) keep[x] |= 0xffu << (8 * y);
             }
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
+            for (int i = 0; i < 4; ++i) {
               uint4& w = ring[st % kRing][i];
               w = make_uint4(w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]);
             }
           }
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
+          for (int i = 0; i < 4; ++i) {
             const uint4 w = ring[st % kRing][i];
             const f16x8_t v0 = codes_f16(w.x, w.y), v1 = codes_f16(w.z, w.w);
-            const int dt = (st - 4) * KS + i;
+            const int dt = (st - KS) * 4 + i;
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) acc[ct][dt] = mfma_f16(v0, p[ct][0], acc[ct][dt]);
 #pragma unroll
@@ -493,84 +501,101 @@ __global__ __launch_bounds__(kThreads, D * CT <= 256 ? 2 : 1) void kv_attention_
     if (m[ct] == -INFINITY && l[ct] != l[ct]) f[ct] = l[ct];  // only scores without a value: they stay NaN
   }
 #pragma unroll
-  for (int w = 0; w < kWaves / kBufs; ++w) {
-    if (kBufs == kWaves || w == wave) {
-      float* buf = red + (kBufs == kWaves ? wave * RT * kPitch : 0);
+  for (int part = 0; part < kParts; ++part) {
+    if (part > 0) __syncthreads();
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
+    for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          f32x4_t* dst = (f32x4_t*)(buf + (ct * 16 + i16) * kPitch + dt * 16 + 4 * g);
-          const f32x4_t v = acc[ct][dt] * f[ct];
-          *dst = kBufs == kWaves || w == 0 ? v : *dst + v;
-        }
-    }
+      for (int dt = 0; dt < DT / kParts; ++dt)
+        *(f32x4_t*)(red + (wave * RT + ct * 16 + i16) * kPitch + dt * 16 + 4 * g) = acc[ct][part * (DT / kParts) + dt] * f[ct];
     __syncthreads();
-  }
-  for (int e = threadIdx.x; e < n_cols * (D / 8); e += kThreads) {
-    const int c = e / (D / 8), d = (e - c * (D / 8)) * 8;
-    float top = -INFINITY, sum = 0.f;
+    for (int e = threadIdx.x; e < n_cols * (DP / 8); e += kThreads) {
+      const int c = e / (DP / 8), dl = (e - c * (DP / 8)) * 8, d = part * DP + dl;
+      float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red_m[w][c]);
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red_m[w][c]);
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      if (red_m[w][c] != -INFINITY) sum += red_l[w][c] * exp2_fast(red_m[w][c] - top);
-    f32x4_t o0 = {0.f, 0.f, 0.f, 0.f}, o1 = o0;
+      for (int w = 0; w < kWaves; ++w)
+        if (red_m[w][c] != -INFINITY) sum += red_l[w][c] * exp2_fast(red_m[w][c] - top);
+      f32x4_t o0 = {0.f, 0.f, 0.f, 0.f}, o1 = o0;
 #pragma unroll
-    for (int w = 0; w < kBufs; ++w) {
-      o0 += *(const f32x4_t*)(red + (w * RT + c) * kPitch + d);
-      o1 += *(const f32x4_t*)(red + (w * RT + c) * kPitch + d + 4);
-    }
-    if (sp.chunks == 1) {
-      const int r = r0 + c, row = r / a.G, head = hk * a.G + (r - row * a.G);
-      uint16_t o[8];
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        o[x] = Qk<F16>::out(o0[x] * inv);
-        o[4 + x] = Qk<F16>::out(o1[x] * inv);
+      for (int w = 0; w < kWaves; ++w) {
+        o0 += *(const f32x4_t*)(red + (w * RT + c) * kPitch + dl);
+        o1 += *(const f32x4_t*)(red + (w * RT + c) * kPitch + dl + 4);
       }
-      *(uint4*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
-          make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
-    } else {
-      float* dst = a.part + ((size_t)blockIdx.x * RT + c) * D + d;
-      *(f32x4_t*)dst = o0;
-      *(f32x4_t*)(dst + 4) = o1;
-      if (d == 0) {
-        float* ml = a.part + (size_t)a.max_items * a.Hk * RT * D + ((size_t)blockIdx.x * RT + c) * 2;
-        ml[0] = top;
-        ml[1] = sum;
+      if (sp.chunks == 1) {
+        const int r = r0 + c, row = r / a.G, head = hk * a.G + (r - row * a.G);
+        uint16_t o[8];
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          o[x] = Qk<F16>::out(o0[x] * inv);
+          o[4 + x] = Qk<F16>::out(o1[x] * inv);
+        }
+        *(uint4*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
+            make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
+      } else {
+        float* dst = a.part + ((size_t)blockIdx.x * RT + c) * D + d;
+        *(f32x4_t*)dst = o0;
+        *(f32x4_t*)(dst + 4) = o1;
+        if (d == 0) {
+          float* ml = a.part + (size_t)a.max_items * a.Hk * RT * D + ((size_t)blockIdx.x * RT + c) * 2;
+          ml[0] = top;
+          ml[1] = sum;
+        }
       }
     }
   }
 }
 
 // Joins the chunks of tiles that were cut: out = sum_c 2^(m_c - m) O_c / sum_c
-// 2^(m_c - m) l_c, in the order of the chunks.  A thread takes four dimensions
-// of a column.
+// 2^(m_c - m) l_c.  A workgroup takes 256 values (64 lanes of four dimensions); its waves take
+// a quarter of the chunks each, and their sums meet in LDS, in order.
 template <int D, int CT, bool F16>
 __global__ __launch_bounds__(kThreads) void kv_attention_join_kernel(AttnArgs a) {
   constexpr int RT = 16 * CT;
+  __shared__ f32x4_t part_o[kWaves][kWave];
+  __shared__ float part_m[kWaves][kWave], part_l[kWaves][kWave];
   const int hk = blockIdx.x % a.Hk;
   Item it;
   if (!find_item<RT>(a, blockIdx.x / a.Hk, true, it)) return;
   const Span sp = span_of<RT>(a, it);
   if (sp.chunks == 1 || it.first_item + sp.chunks > a.max_items) return;
-  const int e = blockIdx.y * kThreads + threadIdx.x;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int n_cols = min(RT, it.rows * a.G - it.tile * RT);
+  for (int e0 = blockIdx.y * kWave; e0 < n_cols * (D / 4); e0 += gridDim.y * kWave) {
+  const int e = e0 + lane;
   const int c = e / (D / 4), d = (e - c * (D / 4)) * 4;
   const int r = it.tile * RT + c;
-  if (c >= RT || r >= it.rows * a.G) return;
+  __syncthreads();  // the sums of the round before are read
   const float* ml = a.part + (size_t)a.max_items * a.Hk * RT * D;
-  float top = -INFINITY;
-  for (int n = 0; n < sp.chunks; ++n) top = fmaxf(top, ml[(((size_t)(it.first_item + n) * a.Hk + hk) * RT + c) * 2]);
-  float sum = 0.f;
+  const int per = (sp.chunks + kWaves - 1) / kWaves, n0 = wave * per, n1 = min(n0 + per, sp.chunks);
+  const size_t at = ((size_t)it.first_item * a.Hk + hk) * RT + c, step = (size_t)a.Hk * RT;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int n = n0; n < n1; ++n) top = fmaxf(top, ml[(at + n * step) * 2]);
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int n = 0; n < sp.chunks; ++n) {
-    const size_t at = ((size_t)(it.first_item + n) * a.Hk + hk) * RT + c;
-    const float mm = ml[at * 2];
-    const float f = mm == -INFINITY ? 0.f : exp2f(mm - top);
-    sum += f * ml[at * 2 + 1];
-    o += f * *(const f32x4_t*)(a.part + at * D + d);
+#pragma unroll 4
+  for (int n = n0; n < n1; ++n) {
+    const float mm = ml[(at + n * step) * 2];
+    const float f = mm == -INFINITY ? 0.f : exp2_fast(mm - top);
+    sum += f * ml[(at + n * step) * 2 + 1];
+    o += f * *(const f32x4_t*)(a.part + (at + n * step) * D + d);
+  }
+  part_o[wave][lane] = o;
+  part_m[wave][lane] = top;
+  part_l[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || c >= n_cols) continue;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, part_m[w][lane]);
+  sum = 0.f;
+  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float mm = part_m[w][lane], f = mm == -INFINITY ? 0.f : exp2_fast(mm - top);
+    sum += f * part_l[w][lane];
+    o += f * part_o[w][lane];
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int row = r / a.G, head = hk * a.G + (r - row * a.G);
@@ -579,6 +604,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_join_kernel(AttnArgs a)
   for (int x = 0; x < 4; ++x) b[x] = Qk<F16>::out(o[x] * inv);
   *(uint2*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
       make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+  }
 }
 
 int after_launch(const char* what) {
@@ -604,7 +630,7 @@ Grid grid_of(int T, int B, int Hq, int Hk, int D) {
   const int RT = 16 * r.ct;
   const int64_t cols = (int64_t)T * G;
   r.max_tiles = (int)(cols < cols / RT + B ? cols : cols / RT + B);
-  r.target = (2 * 256 + Hk - 1) / Hk;
+  r.target = (workgroups_per_cu(D, r.ct) * 256 + Hk - 1) / Hk;
   r.max_items = r.target + r.max_tiles;
   return r;
 }
@@ -618,8 +644,10 @@ bool width_ok(int D) { return D == 64 || D == 128 || D == 256 || D == 512; }
 template <int D, int CT, bool F16>
 void launch(const AttnArgs& a, const Grid& gr, hipStream_t stream) {
   hipLaunchKernelGGL((kv_attention_kernel<D, CT, F16>), dim3(gr.max_items * a.Hk), dim3(kThreads), 0, stream, a);
-  hipLaunchKernelGGL((kv_attention_join_kernel<D, CT, F16>), dim3(gr.max_tiles * a.Hk, (16 * CT * D / 4 + kThreads - 1) / kThreads),
-                     dim3(kThreads), 0, stream, a);
+  // up to 2048 workgroups, each for as many of its tile's values as that leaves
+  const int cols = (int)min((int64_t)16 * CT, (int64_t)(a.q_start ? a.T : 1) * a.G), tiles = gr.max_tiles * a.Hk;
+  const int parts = min(max(2048 / tiles, 1), (cols * (D / 4) + kWave - 1) / kWave);
+  hipLaunchKernelGGL((kv_attention_join_kernel<D, CT, F16>), dim3(tiles, parts), dim3(kThreads), 0, stream, a);
 }
 
 template <int D, bool F16>

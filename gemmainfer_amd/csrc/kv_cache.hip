@@ -241,56 +241,75 @@ __device__ __forceinline__ float page_scale(uint32_t amax_bits) {
 // all: which row lands on each of the page's P places (the last one wins where
 // a slot is named twice), the largest value of those rows, the page's scale,
 // then the codes.  Everything of a page in one workgroup needs no atomics on
-// scales and no second launch.  Reads the rows twice; the second time they
-// come from the caches.  per_wg rows are looked at by one workgroup.
+// scales and no second launch.  A decode step is bound by latency (slots, then
+// rows and scale, then stores), a prompt by HBM; the rows are read twice, the
+// second time from the caches.  per_wg rows are looked at by one workgroup.
 template <typename T, bool kVec>
 __global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
-  __shared__ int last[kMaxPage];
+  __shared__ int last[kMaxPage];               // the row on each place, -1: none
+  __shared__ int place[kMaxPage];              // the places that have one
+  __shared__ uint32_t group_rows[kMaxPage / 16];  // ... as bits of each 16 places
   __shared__ uint32_t wave_max[kAppThreads / kWave];
-  __shared__ int run_end;
-  const int tid = threadIdx.x, head = blockIdx.y, kv = blockIdx.z;
-  const int P = 1 << a.log_page, D = a.D;
+  __shared__ int wave_end[kAppThreads / kWave], wave_count[kAppThreads / kWave];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y, kv = blockIdx.z;
+  const int lp = a.log_page, P = 1 << lp, D = a.D;
   const T* x = (const T*)a.x[kv] + head * a.sh[kv];
   const int64_t st = a.st[kv];
-  const int t_end = min((int)(blockIdx.x + 1) * a.per_wg, a.T);
-  for (int t0 = blockIdx.x * a.per_wg; t0 < t_end; ++t0) {
-    const int64_t slot = a.slots[t0];
-    const int64_t page = slot >> a.log_page;
-    if (slot < 0 || page >= a.num_pages) continue;
-    if (t0 > 0 && a.slots[t0 - 1] >> a.log_page == page) continue;
-    __syncthreads();  // the previous run's readers of LDS are done
-    for (int p = tid; p < P; p += kAppThreads) last[p] = -1;
+  const int t_first = blockIdx.x * a.per_wg;
+  // the first rows of runs among this workgroup's rows (every wave finds them all)
+  unsigned long long runs;
+  {
+    const int t = t_first + lane;
+    const int64_t s = lane < a.per_wg && t < a.T ? a.slots[t] : -1;
+    const int64_t before = t > 0 && t < a.T ? a.slots[t - 1] : -1;
+    runs = __ballot(s >= 0 && s >> lp < a.num_pages && (before < 0 || before >> lp != s >> lp));
+  }
+  for (; runs; runs &= runs - 1) {
+    const int t0 = t_first + __ffsll(runs) - 1;
+    const int64_t page = a.slots[t0] >> lp;
+    float* scale = a.scale[kv] + page * a.Hk + head;
+    const float old = *scale;
+    __syncthreads();  // the run before is done with LDS
+    if (tid < P) last[tid] = -1;
     // ---- the run's rows
     for (int base = t0;; base += kAppThreads) {
-      if (tid == 0) run_end = base + kAppThreads;
-      __syncthreads();
       const int t = base + tid;
       const int64_t s = t < a.T ? a.slots[t] : -1;
-      const bool same = s >= 0 && s >> a.log_page == page;
-      if (!same) atomicMin(&run_end, t);
+      const unsigned long long other = __ballot(s < 0 || s >> lp != page);
+      if (lane == 0) wave_end[wave] = other ? base + wave * kWave + __ffsll(other) - 1 : 0x7fffffff;
       __syncthreads();
-      const int end = run_end;
+      const int end = min(min(wave_end[0], wave_end[1]), min(wave_end[2], wave_end[3]));
       if (t < end) atomicMax(&last[s & (P - 1)], t);
       __syncthreads();
-      if (end < base + kAppThreads) break;
+      if (end != 0x7fffffff) break;
     }
+    const bool on = tid < P && last[tid] >= 0;
+    const unsigned long long bits = __ballot(on);
+    if (lane < 4 && wave * 4 + lane < P >> 4) group_rows[wave * 4 + lane] = (uint32_t)(bits >> (16 * lane)) & 0xffffu;
+    if (lane == 0) wave_count[wave] = __popcll(bits);
+    __syncthreads();
+    int at = __popcll(bits & ((1ull << lane) - 1)), n = 0;
+#pragma unroll
+    for (int w = 0; w < kAppThreads / kWave; ++w) {
+      at += w < wave ? wave_count[w] : 0;
+      n += wave_count[w];
+    }
+    if (on) place[at] = tid;
+    __syncthreads();
     // ---- their largest value
     const int per_row = D >> 3;  // threads of 8 elements
     uint32_t m = 0;
-    for (int i = tid; i < P * per_row; i += kAppThreads) {
-      const int p = i / per_row, c = (i - p * per_row) << 3;
-      const int t = last[p];
-      if (t < 0) continue;
+#pragma unroll 4
+    for (int i = tid; i < n * per_row; i += kAppThreads) {
+      const int r = i / per_row, c = (i - r * per_row) << 3;
       float f[8];
-      load8<T, kVec>(x + t * st + c, f);
+      load8<T, kVec>(x + last[place[r]] * st + c, f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
     }
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, kWave));
-    if ((tid & 63) == 0) wave_max[tid >> 6] = m;
-    float* scale = a.scale[kv] + page * a.Hk + head;
-    const float old = *scale;
+    if (lane == 0) wave_max[wave] = m;
     __syncthreads();
     m = max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]));
     const float need = page_scale(m);
@@ -302,19 +321,23 @@ __global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
     const float inv = valid ? 1.f / now : 0.f;                       // a page without a scale holds zeros
     const bool move = !restart && valid && now > old;
     const float ratio = move ? old * inv : 1.f;
-    uint8_t* codes = a.cache[kv] + (page * a.Hk + head) * ((int64_t)D << a.log_page);
+    uint8_t* codes = a.cache[kv] + (page * a.Hk + head) * ((int64_t)D << lp);
     if (kv == 0) {
-      for (int i = tid; i < P * per_row; i += kAppThreads) {
-        const int p = i / per_row, c = (i - p * per_row) << 3;
-        const int t = last[p];
-        uint2* dst = (uint2*)(codes + (int64_t)p * D + c);
-        if (t >= 0) {
-          float f[8];
-          load8<T, kVec>(x + t * st + c, f);
+#pragma unroll 4
+      for (int i = tid; i < n * per_row; i += kAppThreads) {
+        const int r = i / per_row, c = (i - r * per_row) << 3, p = place[r];
+        float f[8];
+        load8<T, kVec>(x + last[p] * st + c, f);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = valid ? f[j] * inv : 0.f;
-          *dst = make_uint2(pack_e4m3(f[0], f[1], f[2], f[3]), pack_e4m3(f[4], f[5], f[6], f[7]));
-        } else if (move) {
+        for (int j = 0; j < 8; ++j) f[j] = valid ? f[j] * inv : 0.f;
+        *(uint2*)(codes + (int64_t)p * D + c) =
+            make_uint2(pack_e4m3(f[0], f[1], f[2], f[3]), pack_e4m3(f[4], f[5], f[6], f[7]));
+      }
+      if (move) {
+        for (int i = tid; i < P * per_row; i += kAppThreads) {
+          const int p = i / per_row, c = (i - p * per_row) << 3;
+          if (last[p] >= 0) continue;
+          uint2* dst = (uint2*)(codes + (int64_t)p * D + c);
           const uint2 w = *dst;
           *dst = make_uint2(rescale_e4m3(w.x, ratio), rescale_e4m3(w.y, ratio));
         }
@@ -323,33 +346,40 @@ __global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
       // a thread takes one dimension of 16 places: its codes are 16 adjacent bytes
       for (int i = tid; i < D * (P >> 4); i += kAppThreads) {
         const int g = i / D, d = i - g * D;
-        uint8_t* dst = codes + ((int64_t)d << a.log_page) + g * 16;
-        int n_new = 0;
+        const uint32_t rows = group_rows[g];
+        if (rows == 0 && !move) continue;
+        uint8_t* dst = codes + ((int64_t)d << lp) + g * 16;
+        if (rows == 0xffffu || move) {
+          float f[16];
 #pragma unroll
-        for (int p = 0; p < 16; ++p) n_new += last[g * 16 + p] >= 0;
-        if (n_new == 0 && !move) continue;
-        if (n_new == 16 || move) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (n_new < 16) {
-            w = *(const uint4*)dst;
-            w = make_uint4(rescale_e4m3(w.x, ratio), rescale_e4m3(w.y, ratio), rescale_e4m3(w.z, ratio),
-                           rescale_e4m3(w.w, ratio));
+          for (int p = 0; p < 16; ++p) f[p] = Vec8<T>::one(x + max(last[g * 16 + p], t0) * st + d);  // t0: any row
+          uint32_t o[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) f[4 * q + y] = valid ? f[4 * q + y] * inv : 0.f;
+            // a value of no place could be out of range: keep it from the conversion
+#pragma unroll
+            for (int y = 0; y < 4; ++y) f[4 * q + y] = rows >> (4 * q + y) & 1 ? f[4 * q + y] : 0.f;
+            o[q] = pack_e4m3(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
           }
-          uint32_t o[4] = {w.x, w.y, w.z, w.w};
+          if (rows != 0xffffu) {
+            const uint4 w = *(const uint4*)dst;
+            const uint32_t h[4] = {rescale_e4m3(w.x, ratio), rescale_e4m3(w.y, ratio), rescale_e4m3(w.z, ratio),
+                                   rescale_e4m3(w.w, ratio)};
 #pragma unroll
-          for (int p = 0; p < 16; ++p) {
-            const int t = last[g * 16 + p];
-            if (t < 0) continue;
-            const float f = valid ? Vec8<T>::one(x + t * st + d) * inv : 0.f;
-            const uint32_t c = pack_e4m3(f, 0.f, 0.f, 0.f) & 0xffu;
-            o[p >> 2] = (o[p >> 2] & ~(0xffu << (8 * (p & 3)))) | c << (8 * (p & 3));
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t b = rows >> (4 * q) & 0xfu;
+              const uint32_t keep = (b & 1 ? 0xffu : 0u) | (b & 2 ? 0xff00u : 0u) | (b & 4 ? 0xff0000u : 0u) |
+                                    (b & 8 ? 0xff000000u : 0u);
+              o[q] = (o[q] & keep) | (h[q] & ~keep);
+            }
           }
           *(uint4*)dst = make_uint4(o[0], o[1], o[2], o[3]);
         } else {
-          for (int p = 0; p < 16; ++p) {
-            const int t = last[g * 16 + p];
-            if (t < 0) continue;
-            const float f = valid ? Vec8<T>::one(x + t * st + d) * inv : 0.f;
+          for (uint32_t left = rows; left; left &= left - 1) {
+            const int p = __ffs((int)left) - 1;
+            const float f = valid ? Vec8<T>::one(x + last[g * 16 + p] * st + d) * inv : 0.f;
             dst[p] = (uint8_t)pack_e4m3(f, 0.f, 0.f, 0.f);
           }
         }

@@ -44,7 +44,13 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+# The handle of torch's current stream without building a Stream object (2 us of each call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device: torch.device) -> ctypes.c_void_p:
+    if _raw_stream is not None and device.index is not None:
+        return ctypes.c_void_p(_raw_stream(device.index))
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
@@ -56,8 +62,10 @@ def _require(cond: bool, msg: str, exc=ValueError) -> None:
 def _on_device(*tensors: torch.Tensor) -> torch.device:
     dev = tensors[0].device
     for t in tensors:
-        _require(t.is_cuda, "gemmainfer_amd ops take ROCm device tensors only", TypeError)
-        _require(t.device == dev, f"all tensors must be on {dev}, got {t.device}")
+        if not t.is_cuda:
+            raise TypeError("gemmainfer_amd ops take ROCm device tensors only")
+        if t.device != dev:
+            raise ValueError(f"all tensors must be on {dev}, got {t.device}")
     return dev
 
 
@@ -580,11 +588,17 @@ class KVSlots(NamedTuple):
 
 _PAGE_SIZES = (16, 32, 64, 128, 256)
 _HEAD_WIDTHS = (64, 128, 256, 512)
+_ROW_DTYPES = (torch.bfloat16, torch.float16)
 
 
+# A decode step calls these a few times a layer with kernels of microseconds:
+# messages are only formatted where they are raised.
 def _launch_on(device: torch.device):
     """Kernels are launched on the current device: make it the tensors' own."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def kv_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> KVCache:
@@ -601,33 +615,44 @@ def kv_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int, devic
 
 def _cache_shape(cache, who):
     k, v, ks, vs = cache
-    _require(k.dim() == 4 and v.dim() == 4, f"{who}: cache.k is [pages, Hk, page, D], cache.v [pages, Hk, D, page]")
+    if k.dim() != 4:
+        raise ValueError(f"{who}: cache.k must be [pages, Hk, page, D], got {tuple(k.shape)}")
     pages, hk, page, d = k.shape
-    _require(v.shape == (pages, hk, d, page), f"{who}: cache.v must be {(pages, hk, d, page)}, got {tuple(v.shape)}")
-    _require(ks.shape == (pages, hk) and vs.shape == (pages, hk), f"{who}: cache scales must be [pages, Hk]")
-    _require(k.dtype == torch.float8_e4m3fn and v.dtype == torch.float8_e4m3fn,
-             f"{who}: cache.k and cache.v must be float8_e4m3fn", TypeError)
-    _require(ks.dtype == torch.float32 and vs.dtype == torch.float32, f"{who}: cache scales must be fp32", TypeError)
-    _require(k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous(),
-             f"{who}: the cache must be contiguous")
-    _require(page in _PAGE_SIZES, f"{who}: page size must be one of {_PAGE_SIZES}, got {page}")
+    if v.shape != (pages, hk, d, page):
+        raise ValueError(f"{who}: cache.v must be {(pages, hk, d, page)}, got {tuple(v.shape)}")
+    if ks.shape != (pages, hk) or vs.shape != (pages, hk):
+        raise ValueError(f"{who}: cache scales must be [pages, Hk] = {(pages, hk)}")
+    if k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"{who}: cache.k and cache.v must be float8_e4m3fn, got {k.dtype} and {v.dtype}")
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise TypeError(f"{who}: cache scales must be fp32, got {ks.dtype} and {vs.dtype}")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError(f"{who}: the cache must be contiguous")
+    if page not in _PAGE_SIZES:
+        raise ValueError(f"{who}: page size must be one of {_PAGE_SIZES}, got {page}")
     return pages, hk, page, d
 
 
-def _ints(t, name, who, dtype, numel=None):
-    _require(t.dtype == dtype, f"{who}: {name} must be {dtype}, got {t.dtype}", TypeError)
-    _require(t.dim() == 1 and t.is_contiguous(), f"{who}: {name} must be a contiguous vector")
-    _require(numel is None or t.numel() == numel, f"{who}: {name} must have {numel} elements, got {t.numel()}")
+def _vector(t, dtype, who, name, numel=None):
+    if t.dtype != dtype:
+        raise TypeError(f"{who}: {name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{who}: {name} must be a contiguous vector")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{who}: {name} must have {numel} elements, got {t.numel()}")
 
 
 def _table(block_table, batch, who):
-    _require(block_table.dtype == torch.int32, f"{who}: block_table must be int32", TypeError)
-    _require(block_table.dim() == 2 and block_table.shape[0] == batch,
-             f"{who}: block_table must be [B={batch}, pages], got {tuple(block_table.shape)}")
-    cols = block_table.shape[1]
-    _require(cols == 0 or block_table.stride(1) == 1, f"{who}: block_table's rows must be contiguous")
-    _require(batch <= 1 or block_table.stride(0) >= cols, f"{who}: block_table's rows must not overlap")
-    return cols, max(block_table.stride(0), cols)
+    if block_table.dtype != torch.int32:
+        raise TypeError(f"{who}: block_table must be int32, got {block_table.dtype}")
+    if block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise ValueError(f"{who}: block_table must be [B={batch}, pages], got {tuple(block_table.shape)}")
+    cols, (rs, cs) = block_table.shape[1], block_table.stride()
+    if cols > 1 and cs != 1:
+        raise ValueError(f"{who}: block_table's rows must be contiguous")
+    if batch > 1 and rs < cols:
+        raise ValueError(f"{who}: block_table's rows must not overlap")
+    return cols, max(rs, cols)
 
 
 def kv_slots(ctx_lens, new_lens, block_table, free_pages, free_used, page_size, num_rows) -> KVSlots:
@@ -641,25 +666,26 @@ def kv_slots(ctx_lens, new_lens, block_table, free_pages, free_used, page_size, 
     position 0.  A row without a page gets slot -1; ``status`` counts what was
     lacking.  Pass ``status`` as the next step's ``free_used``."""
     dev = _on_device(ctx_lens, new_lens, block_table, free_pages, free_used)
-    _require(ctx_lens.dim() == 1, "kv_slots: ctx_lens must be a vector")
     b = ctx_lens.numel()
-    _ints(ctx_lens, "ctx_lens", "kv_slots", torch.int32)
-    _ints(new_lens, "new_lens", "kv_slots", torch.int32, b)
-    _ints(free_pages, "free_pages", "kv_slots", torch.int32)
-    _ints(free_used, "free_used", "kv_slots", torch.int32)
-    _require(free_used.numel() >= 1, "kv_slots: free_used must have an element")
-    _require(page_size in _PAGE_SIZES, f"kv_slots: page_size must be one of {_PAGE_SIZES}, got {page_size}")
-    _require(0 <= num_rows < 2 ** 31, f"kv_slots: num_rows must be in [0, 2^31), got {num_rows}")
+    _vector(ctx_lens, torch.int32, "kv_slots", "ctx_lens")
+    _vector(new_lens, torch.int32, "kv_slots", "new_lens", b)
+    _vector(free_pages, torch.int32, "kv_slots", "free_pages")
+    _vector(free_used, torch.int32, "kv_slots", "free_used")
+    if free_used.numel() < 1:
+        raise ValueError("kv_slots: free_used must have an element")
+    if page_size not in _PAGE_SIZES:
+        raise ValueError(f"kv_slots: page_size must be one of {_PAGE_SIZES}, got {page_size}")
+    if not 0 <= num_rows < 2 ** 31:
+        raise ValueError(f"kv_slots: num_rows must be in [0, 2^31), got {num_rows}")
     cols, stride = _table(block_table, b, "kv_slots")
-    rows = torch.empty((2, num_rows), dtype=torch.int64, device=dev)
-    ints = torch.empty(2 * b + 4, dtype=torch.int32, device=dev)
-    r = KVSlots(rows[0], rows[1], ints[:b + 1], ints[b + 1:2 * b + 1], ints[2 * b + 1:])
+    slots, positions = torch.empty((2, num_rows), dtype=torch.int64, device=dev).unbind(0)
+    q_start, seq_lens, status = torch.empty(2 * b + 4, dtype=torch.int32, device=dev).split((b + 1, b, 3))
     with _launch_on(dev):
         L.check(L.load().gi_kv_slots(
-            _ptr(ctx_lens), _ptr(new_lens), b, _ptr(block_table), cols, stride, _ptr(free_pages),
-            free_pages.numel(), _ptr(free_used), int(page_size), _ptr(r.slots), _ptr(r.positions), int(num_rows),
-            _ptr(r.q_start), _ptr(r.seq_lens), _ptr(r.status), _stream(dev)), "kv_slots")
-    return r
+            ctx_lens.data_ptr(), new_lens.data_ptr(), b, block_table.data_ptr(), cols, stride, free_pages.data_ptr(),
+            free_pages.numel(), free_used.data_ptr(), page_size, slots.data_ptr(), positions.data_ptr(), num_rows,
+            q_start.data_ptr(), seq_lens.data_ptr(), status.data_ptr(), _stream(dev)), "kv_slots")
+    return KVSlots(slots, positions, q_start, seq_lens, status)
 
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0,
@@ -701,37 +727,44 @@ def rope_rows(q, k, positions, inv_freq, *, interleaved: bool = False, mscale: f
     per rotated pair: the first 2 * len(inv_freq) dimensions turn, pair i being
     (i, i + len) or, ``interleaved``, (2i, 2i + 1); the others are kept.
     ``mscale`` multiplies cos and sin."""
-    dev = _on_device(q, positions, inv_freq)
-    _require(q.dtype in _ACT_DTYPES, "rope_rows: bf16/fp16/fp32 only", TypeError)
-    _require(q.dim() == 3, f"rope_rows: q must be [T, Hq, D], got {tuple(q.shape)}")
+    dev = _on_device(q, positions, inv_freq) if k is None else _on_device(q, k, positions, inv_freq)
+    if q.dtype not in _ACT_DTYPES:
+        raise TypeError(f"rope_rows: bf16/fp16/fp32 only, got {q.dtype}")
+    if q.dim() != 3:
+        raise ValueError(f"rope_rows: q must be [T, Hq, D], got {tuple(q.shape)}")
     t, hq, d = q.shape
-    _require(q.stride(2) == 1 or d == 1, "rope_rows: q's last dimension must be contiguous")
+    qs = q.stride()
+    if qs[2] != 1 and d > 1:
+        raise ValueError("rope_rows: q's last dimension must be contiguous")
+    hk, ks = 0, (0, 0)
     if k is not None:
-        _on_device(q, k)
-        _require(k.dim() == 3 and k.shape[0] == t and k.shape[2] == d and k.dtype == q.dtype,
-                 "rope_rows: k must be [T, Hk, D] like q")
-        _require(k.stride(2) == 1 or d == 1, "rope_rows: k's last dimension must be contiguous")
-    _ints(positions, "positions", "rope_rows", torch.int64, t)
-    _require(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(),
-             "rope_rows: inv_freq must be a contiguous fp64 vector", TypeError)
+        if k.dim() != 3 or k.shape[0] != t or k.shape[2] != d or k.dtype != q.dtype:
+            raise ValueError(f"rope_rows: k must be [{t}, Hk, {d}] of q's dtype, got {tuple(k.shape)} {k.dtype}")
+        hk, ks = k.shape[1], k.stride()
+        if ks[2] != 1 and d > 1:
+            raise ValueError("rope_rows: k's last dimension must be contiguous")
+    _vector(positions, torch.int64, "rope_rows", "positions", t)
+    _vector(inv_freq, torch.float64, "rope_rows", "inv_freq")
     rot = 2 * inv_freq.numel()
-    _require(0 < rot <= d, f"rope_rows: {inv_freq.numel()} frequencies rotate {rot} of {d} dimensions")
+    if not 0 < rot <= d:
+        raise ValueError(f"rope_rows: {inv_freq.numel()} frequencies rotate {rot} of {d} dimensions")
     if inplace:
-        qo, ko = q, k
+        qo, ko, qos, kos = q, k, qs, ks
         for name, x in (("q", q), ("k", k)):
-            _require(x is None or x.numel() == 0 or all(s > 0 or n == 1 for s, n in zip(x.stride(), x.shape)),
-                     f"rope_rows: {name} has broadcast dimensions, which cannot be rotated in place")
+            if x is not None and any(st == 0 and n > 1 for st, n in zip(x.stride(), x.shape)):
+                raise ValueError(f"rope_rows: {name} has broadcast dimensions, which cannot be rotated in place")
     else:
         qo = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
-        ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+        qos = (hq * d, d)
+        ko = None if k is None else torch.empty((t, hk, d), dtype=q.dtype, device=dev)
+        kos = (hk * d, d)
     if t == 0:
         return qo, ko
-    ks, kos = ((0, 0), (0, 0)) if k is None else (k.stride(), ko.stride())
     with _launch_on(dev):
         L.check(L.load().gi_rope_rows(
-            _ptr(q), _ptr(qo), _ptr(k), _ptr(ko), _ptr(positions), _ptr(inv_freq), _DTYPE_CODE[q.dtype], t, hq,
-            0 if k is None else k.shape[1], d, rot, int(bool(interleaved)), float(mscale), q.stride(0), q.stride(1),
-            qo.stride(0), qo.stride(1), ks[0], ks[1], kos[0], kos[1], _stream(dev)), "rope_rows")
+            q.data_ptr(), qo.data_ptr(), None if k is None else k.data_ptr(), None if k is None else ko.data_ptr(),
+            positions.data_ptr(), inv_freq.data_ptr(), _DTYPE_CODE[q.dtype], t, hq, hk, d, rot, bool(interleaved),
+            mscale, qs[0], qs[1], qos[0], qos[1], ks[0], ks[1], kos[0], kos[1], _stream(dev)), "rope_rows")
     return qo, ko
 
 
@@ -740,28 +773,33 @@ def kv_append(k, v, slots, cache: KVCache) -> None:
     (int64 [T]; negative ones, and those past the last page, are skipped).
 
     The rows of one page must follow each other, as those of a request do; of
-    rows with the same slot the last one is stored.  Each page has one scale per head for K and one for V,
-    a power of two that grows as larger rows arrive (what the page holds is
-    then rounded to the new one); writing a page's first place starts the page
-    anew.  A row with an infinity or NaN makes its page's scale NaN until then."""
+    rows with the same slot the last one is stored.  Each page has one scale per
+    head for K and one for V, a power of two that grows as larger rows arrive
+    (what the page holds is then rounded to the new one); writing a page's first
+    place starts the page anew.  A row with an infinity or NaN makes its page's
+    scale NaN until then."""
     dev = _on_device(k, v, slots, *cache)
     pages, hk, page, d = _cache_shape(cache, "kv_append")
-    _require(k.dtype in _ACT_DTYPES and v.dtype == k.dtype, "kv_append: k and v must be bf16, fp16 or fp32, alike",
-             TypeError)
-    _require(k.dim() == 3 and k.shape[1:] == (hk, d) and v.shape == k.shape,
-             f"kv_append: k and v must be [T, {hk}, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    _require(k.stride(2) == 1 and v.stride(2) == 1, "kv_append: the last dimension of k and v must be contiguous")
-    t = k.shape[0]
-    _ints(slots, "slots", "kv_append", torch.int64, t)
+    if k.dtype not in _ACT_DTYPES or v.dtype != k.dtype:
+        raise TypeError(f"kv_append: k and v must be bf16, fp16 or fp32, alike; got {k.dtype} and {v.dtype}")
+    t = slots.numel()
+    if k.shape != (t, hk, d) or v.shape != k.shape:
+        raise ValueError(f"kv_append: k and v must be [{t}, {hk}, {d}] (one row a slot), got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or vs[2] != 1:
+        raise ValueError("kv_append: the last dimension of k and v must be contiguous")
+    _vector(slots, torch.int64, "kv_append", "slots")
     with _launch_on(dev):
         L.check(L.load().gi_kv_append(
-            _ptr(k), _ptr(v), _DTYPE_CODE[k.dtype], k.stride(0), k.stride(1), v.stride(0), v.stride(1), _ptr(slots),
-            t, hk, d, page, pages, _ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale),
+            k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), t, hk, d,
+            page, pages, cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(),
             _stream(dev)), "kv_append")
 
 
 def _rows_aligned(x):
-    return x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.data_ptr() % 16 == 0
+    s = x.stride()
+    return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and x.data_ptr() % 16 == 0
 
 
 def _overlap(x, y):
@@ -785,43 +823,50 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
     head h reads kv head h // (Hq // Hk).  Rows behind the last request are not
     computed: they keep what ``out`` holds, and are unspecified without it.  A
     row that sees a token without a page (outside the cache, or past the table) gets NaN."""
-    dev = _on_device(q, block_table, seq_lens, *cache)
-    pages, hk, page, d = _cache_shape(cache, "kv_attention")
-    _require(q.dtype in (torch.bfloat16, torch.float16), f"kv_attention: q must be bf16 or fp16, got {q.dtype}",
-             TypeError)
-    _require(q.dim() == 3 and q.shape[2] == d and q.shape[1] % hk == 0 and q.shape[1] > 0,
-             f"kv_attention: q must be [T, a multiple of {hk}, {d}], got {tuple(q.shape)}")
-    _require(d in _HEAD_WIDTHS, f"kv_attention: head width must be one of {_HEAD_WIDTHS}, got {d}")
-    t, hq, _ = q.shape
-    _require(seq_lens.dim() == 1, "kv_attention: seq_lens must be a vector")
-    b = seq_lens.numel()
-    _ints(seq_lens, "seq_lens", "kv_attention", torch.int32)
-    cols, stride = _table(block_table, b, "kv_attention")
     if q_start is None:
-        _require(t == b, f"kv_attention: without q_start there is one row a request: {t} rows, {b} requests")
+        dev = _on_device(q, block_table, seq_lens, *cache)
     else:
-        _on_device(q, q_start)
-        _ints(q_start, "q_start", "kv_attention", torch.int32, b + 1)
-    _require(int(window) >= 0, f"kv_attention: window must be >= 0 (0: none), got {window}")
+        dev = _on_device(q, block_table, seq_lens, q_start, *cache)
+    pages, hk, page, d = _cache_shape(cache, "kv_attention")
+    if q.dtype not in _ROW_DTYPES:
+        raise TypeError(f"kv_attention: q must be bf16 or fp16, got {q.dtype}")
+    if q.dim() != 3 or q.shape[2] != d or q.shape[1] % hk or q.shape[1] == 0:
+        raise ValueError(f"kv_attention: q must be [T, a multiple of {hk}, {d}], got {tuple(q.shape)}")
+    if d not in _HEAD_WIDTHS:
+        raise ValueError(f"kv_attention: head width must be one of {_HEAD_WIDTHS}, got {d}")
+    t, hq, _ = q.shape
+    b = seq_lens.numel()
+    _vector(seq_lens, torch.int32, "kv_attention", "seq_lens")
+    cols, stride = _table(block_table, b, "kv_attention")
+    if q_start is not None:
+        _vector(q_start, torch.int32, "kv_attention", "q_start", b + 1)
+    elif t != b:
+        raise ValueError(f"kv_attention: without q_start there is one row a request: {t} rows, {b} requests")
+    if window < 0:
+        raise ValueError(f"kv_attention: window must be >= 0 (0: none), got {window}")
     if out is None:
         out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+        os = (hq * d, d)
     else:
         _on_device(q, out)
-        _require(out.shape == q.shape and out.dtype == q.dtype and _rows_aligned(out),
-                 "kv_attention: out must be like q, its rows contiguous and 16-byte aligned")
-        _require(not _overlap(q, out), "kv_attention: out must not overlap q")
+        if out.shape != q.shape or out.dtype != q.dtype or not _rows_aligned(out):
+            raise ValueError("kv_attention: out must be like q, its rows contiguous and 16-byte aligned")
+        if _overlap(q, out):
+            raise ValueError("kv_attention: out must not overlap q")
+        os = out.stride()
     if t == 0 or b == 0:
         return out
     if not _rows_aligned(q):
         q = q.clone(memory_format=torch.contiguous_format)
+    qs = q.stride()
     lib = L.load()
     nbytes = lib.gi_kv_attention_workspace_bytes(t, b, hq, hk, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _launch_on(dev):
         L.check(lib.gi_kv_attention(
-            _ptr(q), _DTYPE_CODE[q.dtype], q.stride(0), q.stride(1), _ptr(cache.k), _ptr(cache.v),
-            _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(block_table), cols, stride, _ptr(seq_lens),
-            _ptr(q_start), _ptr(out), out.stride(0), out.stride(1), t, b, hq, hk, d, page, pages,
-            float(d ** -0.5 if scale is None else scale), int(window), _ptr(ws), nbytes, _stream(dev)),
+            q.data_ptr(), _DTYPE_CODE[q.dtype], qs[0], qs[1], cache[0].data_ptr(), cache[1].data_ptr(),
+            cache[2].data_ptr(), cache[3].data_ptr(), block_table.data_ptr(), cols, stride, seq_lens.data_ptr(),
+            None if q_start is None else q_start.data_ptr(), out.data_ptr(), os[0], os[1], t, b, hq, hk, d, page,
+            pages, d ** -0.5 if scale is None else scale, window, ws.data_ptr(), nbytes, _stream(dev)),
             "kv_attention")
     return out
