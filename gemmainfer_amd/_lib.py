@@ -91,7 +91,7 @@ SIGNATURES = {
                             c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "gi_kv_append": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int, c_int,
                              c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "gi_kv_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "gi_kv_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int64]),
     "gi_kv_attention": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int,
                                 c_int, c_int, c_int, c_int64, c_float, c_int, c_void_p, c_size_t, c_void_p]),

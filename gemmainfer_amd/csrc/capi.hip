@@ -378,8 +378,8 @@ int gi_kv_append(const void* k, const void* v, int dtype, int64_t k_st, int64_t 
                               v_scale, as_stream(stream));
 }
 
-size_t gi_kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D) {
-  return gi::kv_attention_workspace_bytes(T, B, Hq, Hk, D);
+size_t gi_kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D, int64_t max_tokens) {
+  return gi::kv_attention_workspace_bytes(T, B, Hq, Hk, D, max_tokens);
 }
 
 int gi_kv_attention(const void* q, int dtype, int64_t q_st, int64_t q_sh, const void* k_cache, const void* v_cache,

@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void rope_kernel(T* q, T* k, const T* cs, cons
 // of each half) of one head of one row; a workgroup the units of one row, whose cos and
 // sin its threads work out once, into LDS, while their elements are on the way.  Bound by HBM: each
 // element is read and written once.
-constexpr int kRopeThreads = 1024;  // at most
+constexpr int kRopeThreads = 256;
 constexpr int kRopeMaxPairs = 512;
 
 struct RopeArgs {
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs a) {
   __shared__ float cs[kRopeMaxPairs], sn[kRopeMaxPairs];
   const int64_t row = blockIdx.x;
   const int R = 2 * a.pairs;
-  const int i = blockIdx.y * blockDim.x + threadIdx.x;
+  const int i = blockIdx.y * kRopeThreads + threadIdx.x;
   const int h = i / a.units, u = i - h * a.units;
   const bool on = h < a.heads[0] + a.heads[1], turns = u < a.turn;
   const int w = h < a.heads[0] ? 0 : 1, hw = h - (w ? a.heads[0] : 0);
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs a) {
     if (two) v2 = *(const Pack<T, N>*)(x + d2);
   }
   const double p = (double)a.pos[row];
-  for (int j = threadIdx.x; j < a.pairs; j += blockDim.x) {
+  for (int j = threadIdx.x; j < a.pairs; j += kRopeThreads) {
     const double t = p * a.freq[j] * 0.15915494309189535;  // 1 / (2 pi)
     const float r = (float)(t - rint(t));
     float s, c;
@@ -286,17 +286,15 @@ int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, con
   const bool copy = (Hq > 0 && q != q_out) || (Hk > 0 && k != k_out);
   a.turn = !vec ? a.pairs : interleaved ? rotary_dim / 8 : rotary_dim / 16;
   a.units = a.turn + (copy ? (D - rotary_dim) / (vec ? 8 : 1) : 0);
-  // few rows are spread over workgroups of 256; of many, each row is one workgroup where it fits
-  // (2047 rows of 16 + 8 heads of 256: 12.6 us in workgroups of 256, which work the row's angles out twice)
-  const int64_t all = (int64_t)(Hq + Hk) * a.units;
-  const int threads = T < 256 ? 256 : (int)(all < kRopeThreads ? (all + 63) / 64 * 64 : kRopeThreads);
-  const int64_t parts = (all + threads - 1) / threads;
+  // (two units a thread, or a whole row in one workgroup: within 0.5 us for
+  // 2047 rows of 16 + 8 heads of 256, 12.3 us)
+  const int64_t parts = ((int64_t)(Hq + Hk) * a.units + kRopeThreads - 1) / kRopeThreads;
   if (parts > 65535) return fail(GI_ERR_UNSUPPORTED, "rope_rows: too many heads");
   const dim3 grid(T, (unsigned)parts);
 #define GI_ROPE_V(T_, I_)                                                                                 \
   do {                                                                                                    \
-    if (vec) hipLaunchKernelGGL((rope_rows_kernel<T_, I_, true>), grid, dim3(threads), 0, stream, a);  \
-    else hipLaunchKernelGGL((rope_rows_kernel<T_, I_, false>), grid, dim3(threads), 0, stream, a);     \
+    if (vec) hipLaunchKernelGGL((rope_rows_kernel<T_, I_, true>), grid, dim3(kRopeThreads), 0, stream, a);  \
+    else hipLaunchKernelGGL((rope_rows_kernel<T_, I_, false>), grid, dim3(kRopeThreads), 0, stream, a);     \
   } while (0)
 #define GI_ROPE_I(T_)                 \
   do {                                \

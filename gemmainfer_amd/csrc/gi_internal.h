@@ -176,7 +176,7 @@ int launch_kv_slots(const int32_t* ctx_lens, const int32_t* new_lens, int B, int
 int launch_kv_append(const void* k, const void* v, int dtype, const int64_t* k_strides, const int64_t* v_strides,
                      const int64_t* slots, int T, int Hk, int D, int page_size, int64_t num_pages, void* k_cache,
                      void* v_cache, float* k_scale, float* v_scale, hipStream_t stream);
-size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D);
+size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D, int64_t max_tokens);
 int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, const void* k_cache, const void* v_cache,
                         const float* k_scale, const float* v_scale, const int32_t* block_table, int64_t table_stride,
                         int max_pages, const int32_t* seq_lens, const int32_t* q_start, void* out,

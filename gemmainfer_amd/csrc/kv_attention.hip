@@ -27,9 +27,9 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kUnit = 64;      // cache rows a wave takes at a time
 constexpr int kMinChunk = 4;   // units: one a wave
-constexpr int kFree = 0x8f;
+constexpr int kRounds = 4;
 // what a compute unit holds of a kernel: by its registers, two waves a SIMD or one
-constexpr int workgroups_per_cu(int D, int CT) { return D * CT <= 256 && CT <= 2 ? 2 : 1; }
+constexpr int workgroups_per_cu(int D, int CT) { return D * CT <= (CT == 1 ? 256 : 128) ? 2 : 1; }
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights go to the matrix cores in fp16 as 2^(t - m + kBias), at most 2^(kBias
 // + kSlack): fp16 is normal down to 2^-14, so a weight 2^-21 of the largest
@@ -49,10 +49,12 @@ struct AttnArgs {
   const int32_t* q_start;  // null: one row a request
   void* out;
   int64_t o_st, o_sh;
-  float* part;             // [items * Hk][RT][D] partial sums, then [items * Hk][RT] (maximum, sum)
+  float* part;             // [max_slots * Hk][RT][D] partial sums, then [max_slots * Hk][RT] (maximum, sum)
   int64_t num_pages;
   float scale;             // with log2(e)
-  int T, B, Hk, G, cols, log_page, window, target, max_items;
+  int T, B, Hk, G, cols, log_page, window;
+  int resident;            // workgroups of a kv head that the chip holds at a time
+  int max_slots;
 };
 
 // ---------------------------------------------------------------------------
@@ -64,11 +66,20 @@ struct AttnArgs {
 // chunk is the same for all requests: a long one is shared by as many
 // workgroups as a batch of short ones.
 struct Item {
-  int b, tile, tiles, chunk_no, chunk, q0, rows, len, first_item;
+  int b, tile, chunk_no, chunk, q0, rows, len;
+  int slot;   // of the tile's first partial sum, among those of one kv head
   bool over;  // longer than the table: its pages cannot all be there
 };
 
-struct Load {
+// The lane, worked out anew: what hangs on it in the loop over items is not
+// kept in registers from one to the next.
+__device__ __forceinline__ int this_lane() {
+  int v = threadIdx.x & 63;
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+struct Load {  // of one request
   int q0, rows, len, tiles, units;
   bool over;
 };
@@ -82,21 +93,19 @@ __device__ __forceinline__ Load load_of(const AttnArgs& a, int b) {
     q0 = min(max(a.q_start[b], 0), a.T);
     q1 = min(max(a.q_start[b + 1], q0), a.T);
   }
-  const int64_t cap = (int64_t)a.cols << a.log_page;
-  const int64_t len = max(a.lens[b], 0);
+  const int cap = a.cols << a.log_page;  // at most 2^30
+  const int len = max(a.lens[b], 0);
   r.q0 = q0;
   r.rows = q1 - q0;
   r.over = len > cap;
-  r.len = (int)min(len, cap);
-  r.tiles = (int)(((int64_t)r.rows * a.G + RT - 1) / RT);
-  int units = (r.len + kUnit - 1) / kUnit;
-  if (a.window > 0) units = (int)min((int64_t)units, ((int64_t)a.window + RT) / kUnit + 2);
-  r.units = units;
+  r.len = min(len, cap);
+  r.tiles = (r.rows * a.G + RT - 1) / RT;  // rows * G at most 2^30
+  r.units = (r.len + kUnit - 1) / kUnit;
+  if (a.window > 0 && a.window <= cap) r.units = min(r.units, (a.window + RT) / kUnit + 2);
   return r;
 }
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) {
     const int u = __shfl_up(v, off, kWave);
@@ -105,51 +114,85 @@ __device__ __forceinline__ int wave_scan(int v) {  // inclusive
   return v;
 }
 
-// Item `want` of the list (by_tile: the first item of tile `want`); false past its end.
+template <typename N>
+__device__ __forceinline__ N wave_sum(N v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+// The chunk, in units: `total` tile units of a kv head go to `resident`
+// workgroups that the chip holds at a time, in k = 1 ... 4 rounds.  One round
+// is best where the chunks come out even (a few long requests: two of 70001 and 130005
+// tokens 77 us in one round, 91 in two), several where many requests of
+// other lengths leave workgroups idle (47 up to 8190 tokens: 214, 202 and 194 us in one,
+// two and three).  k is the one with the least estimate: rounds of whole
+// chunks, or what any order of work stays under, and two units to start each round.
 template <int RT>
-__device__ __forceinline__ bool find_item(const AttnArgs& a, int want, bool by_tile, Item& it) {
+__device__ __forceinline__ int chunk_of(const AttnArgs& a) {
   const int lane = threadIdx.x & 63;
   const Load head = load_of<RT>(a, lane);
-  long long total = 0;
+  double total = 0.;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
     const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
-    total += (long long)l.tiles * l.units;
+    total += (double)l.tiles * l.units;
   }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, kWave);
-  int chunk = (int)max((total + a.target - 1) / a.target, (long long)kMinChunk);
-  chunk = (chunk + kWaves - 1) / kWaves * kWaves;
-  int items = 0, tiles = 0;
+  total = wave_sum(total);
+  int best = 0;
+  float least = 0.f;
+#pragma unroll 1
+  for (int k = 1; k <= kRounds; ++k) {
+    int c = (int)(total / ((double)a.resident * k)) + 1;
+    c = (max(c, kMinChunk) + kWaves - 1) / kWaves * kWaves;
+    if (k > 1 && c >= best) break;
+    int items = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kWave) {
+      const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
+      items += l.tiles * ((l.units + c - 1) / c);
+    }
+    items = wave_sum(items);
+    const int rounds = (items + a.resident - 1) / a.resident;
+    const float cost = fminf((float)rounds * c, (float)(total / a.resident) + c) + 2.f * rounds;
+    if (k == 1 || cost < least) {
+      best = c;
+      least = cost;
+    }
+    if (c <= 4 * kMinChunk) break;
+  }
+  return __builtin_amdgcn_readfirstlane(best);
+}
+
+// Item `want` of the list (by_tile: the first item of tile `want`); false past its end.
+template <int RT>
+__device__ __forceinline__ bool find_item(const AttnArgs& a, int chunk, int want, bool by_tile, Item& it) {
+  const int lane = this_lane();
+  int items = 0, tiles = 0, slots = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
-    const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
+    const Load l = load_of<RT>(a, b0 + lane);
     const int chunks = max((l.units + chunk - 1) / chunk, 1);
-    const int n = l.tiles * chunks;
-    const int item_end = items + wave_scan(n), tile_end = tiles + wave_scan(l.tiles);
-    const int end = by_tile ? tile_end : item_end, first = end - (by_tile ? l.tiles : n);
-    const unsigned long long hit = __ballot(want >= first && want < end);
+    const int n = l.tiles * chunks, n_slots = chunks > 1 ? n : 0;
+    const int count = by_tile ? l.tiles : n;
+    const int end = (by_tile ? tiles : items) + wave_scan(count, lane), slot_end = slots + wave_scan(n_slots, lane);
+    const unsigned long long hit = __ballot(want >= end - count && want < end);
     if (hit) {
       const int src = __ffsll(hit) - 1;
-      const int in = want - __shfl(first, src, kWave);
-      const int per = __shfl(chunks, src, kWave);
-      const int first_item = __shfl(item_end - n, src, kWave);
+      auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
+      const int in = want - pick(end - count), per = pick(chunks);
       it.b = b0 + src;
       it.tile = by_tile ? in : in / per;
       it.chunk_no = by_tile ? 0 : in - it.tile * per;
-      it.tiles = __shfl(l.tiles, src, kWave);
       it.chunk = chunk;
-      it.q0 = __shfl(l.q0, src, kWave);
-      it.rows = __shfl(l.rows, src, kWave);
-      it.len = __shfl(l.len, src, kWave);
-      it.over = __shfl((int)l.over, src, kWave);
-      it.first_item = first_item + it.tile * per;
+      it.q0 = pick(l.q0);
+      it.rows = pick(l.rows);
+      it.len = pick(l.len);
+      it.over = pick((int)l.over);
+      it.slot = pick(slot_end - n_slots) + it.tile * per;
       // the last tiles of a prompt see the most: they go first
-      it.tile = it.tiles - 1 - it.tile;
-      for (int* f : {&it.b, &it.tile, &it.tiles, &it.chunk_no, &it.chunk, &it.q0, &it.rows, &it.len, &it.first_item})
-        *f = __builtin_amdgcn_readfirstlane(*f);
+      it.tile = pick(l.tiles) - 1 - it.tile;
       return true;
     }
-    items = __shfl(item_end, kWave - 1, kWave);
-    tiles = __shfl(tile_end, kWave - 1, kWave);
+    (by_tile ? tiles : items) = __builtin_amdgcn_readlane(end, kWave - 1);
+    slots = __builtin_amdgcn_readlane(slot_end, kWave - 1);
   }
   return false;
 }
@@ -163,9 +206,9 @@ struct Span {
 template <int RT>
 __device__ __forceinline__ Span span_of(const AttnArgs& a, const Item& it) {
   Span s;
-  const int64_t r0 = (int64_t)it.tile * RT, r1 = min(r0 + RT, (int64_t)it.rows * a.G) - 1;
-  s.pos_min = it.len - it.rows + (int)(r0 / a.G);
-  s.pos_max = it.len - it.rows + (int)(r1 / a.G);
+  const int r0 = it.tile * RT, r1 = min(r0 + RT, it.rows * a.G) - 1;
+  s.pos_min = it.len - it.rows + r0 / a.G;
+  s.pos_max = it.len - it.rows + r1 / a.G;
   s.lo = 0;
   if (a.window > 0) s.lo = max(s.pos_min - a.window + 1, 0) / kUnit;
   s.hi = s.pos_max < 0 ? 0 : s.pos_max / kUnit + 1;
@@ -272,6 +315,10 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
   // the waves' sums meet in LDS, a part of the dimensions at a time where they do not fit together
   constexpr int kParts = (size_t)RT * (D + 4) * kWaves * 4 <= 140000 ? 1 : 2;
   constexpr int DP = D / kParts, kPitch = DP + 4;
+  // What may move over a step's loads: nothing, or where a compute unit holds
+  // two workgroups all that is no memory access (16 columns of 256: 186 us
+  // instead of 220, of 512 the other way 80.5 instead of 82.7, 64 of 256 278 instead of 294)
+  constexpr int kFree = workgroups_per_cu(D, CT) > 1 ? 0x8f : 0;
   constexpr size_t kRedBytes = (size_t)kWaves * RT * kPitch * 4, kQBytes = kQLds ? (size_t)CT * 2 * KS * kWave * 16 : 16;
   typedef typename Qk<F16>::frag frag;
   __shared__ __align__(16) char lds[kRedBytes > kQBytes ? kRedBytes : kQBytes];
@@ -279,16 +326,19 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
   uint4* q_lds = (uint4*)lds;
   float* red = (float*)lds;
 
+  const int wave = uniform(threadIdx.x >> 6);
   const int hk = blockIdx.x % a.Hk;
+  const int chunk = chunk_of<RT>(a);
   Item it;
-  if (!find_item<RT>(a, blockIdx.x / a.Hk, false, it)) return;
+  for (int want = blockIdx.x / a.Hk; find_item<RT>(a, chunk, want, false, it); want += gridDim.x / a.Hk) {
   const Span sp = span_of<RT>(a, it);
-  if (it.chunk_no >= sp.chunks) return;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  if (it.chunk_no >= sp.chunks || (sp.chunks > 1 && it.slot + sp.chunks > a.max_slots)) continue;
+  __syncthreads();  // the item before is done with LDS
+  const int lane = this_lane();
   const int i16 = lane & 15, g = lane >> 4;
   const int page_mask = (1 << a.log_page) - 1;
   const int r0 = it.tile * RT;
-  const int n_cols = (int)min((int64_t)RT, (int64_t)it.rows * a.G - r0);
+  const int n_cols = min(RT, it.rows * a.G - r0);
 
   // ---- Q as operand B: column i, dimensions 64 s + 16 g + 8 h ... of step 2 s + h
   frag qf[kQLds ? 1 : CT][kQLds ? 1 : 2 * KS];
@@ -369,6 +419,7 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
       const bool edge = tok + kUnit - 1 > pos_min || (a.window > 0 && tok <= pos_max - a.window);
       f32x4_t s[CT][4];
       f16x8_t p[CT][2];
+      uint32_t keep[4];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -443,20 +494,22 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
             // rows that are not seen weigh nothing, whatever their page's scale is
             l[ct] += sum == 0.f ? 0.f : sum * inv_vs;
           }
-        }
-        if (st >= KS) {
-          // ---- O^T += V^T P^T, 64 dimensions
-          if (edge) {  // rows that no column sees may hold anything
-            const int last = min(pos_max - (tok + 16 * g), 15);
-            const int first = a.window > 0 ? pos_min - a.window + 1 - (tok + 16 * g) : 0;
-            uint32_t keep[4];
+          // rows of V that no column sees may hold anything
+          const int last = min(pos_max - (tok + 16 * g), 15);
+          const int first = a.window > 0 ? pos_min - a.window + 1 - (tok + 16 * g) : 0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              keep[x] = 0;
+          for (int x = 0; x < 4; ++x) {
+            keep[x] = 0;
+            if (edge) {
 #pragma unroll
               for (int y = 0; y < 4; ++y)
                 if (4 * x + y <= last && 4 * x + y >= first) keep[x] |= 0xffu << (8 * y);
             }
+          }
+        }
+        if (st >= KS) {
+          // ---- O^T += V^T P^T, 64 dimensions
+          if (edge) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint4& w = ring[st % kRing][i];
@@ -535,75 +588,78 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
         *(uint4*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
             make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
       } else {
-        float* dst = a.part + ((size_t)blockIdx.x * RT + c) * D + d;
+        const size_t at = ((size_t)(it.slot + it.chunk_no) * a.Hk + hk) * RT + c;
+        float* dst = a.part + at * D + d;
         *(f32x4_t*)dst = o0;
         *(f32x4_t*)(dst + 4) = o1;
         if (d == 0) {
-          float* ml = a.part + (size_t)a.max_items * a.Hk * RT * D + ((size_t)blockIdx.x * RT + c) * 2;
+          float* ml = a.part + (size_t)a.max_slots * a.Hk * RT * D + at * 2;
           ml[0] = top;
           ml[1] = sum;
         }
       }
     }
   }
+  }
 }
 
 // Joins the chunks of tiles that were cut: out = sum_c 2^(m_c - m) O_c / sum_c
-// 2^(m_c - m) l_c.  A workgroup takes 256 values (64 lanes of four dimensions); its waves take
-// a quarter of the chunks each, and their sums meet in LDS, in order.
+// 2^(m_c - m) l_c.  A workgroup takes 256 values at a time (64 lanes of four
+// dimensions); its waves take a quarter of the chunks each, and their sums meet
+// in LDS, in order.
 template <int D, int CT, bool F16>
 __global__ __launch_bounds__(kThreads) void kv_attention_join_kernel(AttnArgs a) {
   constexpr int RT = 16 * CT;
   __shared__ f32x4_t part_o[kWaves][kWave];
   __shared__ float part_m[kWaves][kWave], part_l[kWaves][kWave];
   const int hk = blockIdx.x % a.Hk;
+  const int chunk = chunk_of<RT>(a);
   Item it;
-  if (!find_item<RT>(a, blockIdx.x / a.Hk, true, it)) return;
+  if (!find_item<RT>(a, chunk, blockIdx.x / a.Hk, true, it)) return;
   const Span sp = span_of<RT>(a, it);
-  if (sp.chunks == 1 || it.first_item + sp.chunks > a.max_items) return;
+  if (sp.chunks == 1 || it.slot + sp.chunks > a.max_slots) return;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n_cols = min(RT, it.rows * a.G - it.tile * RT);
-  for (int e0 = blockIdx.y * kWave; e0 < n_cols * (D / 4); e0 += gridDim.y * kWave) {
-  const int e = e0 + lane;
-  const int c = e / (D / 4), d = (e - c * (D / 4)) * 4;
-  const int r = it.tile * RT + c;
-  __syncthreads();  // the sums of the round before are read
-  const float* ml = a.part + (size_t)a.max_items * a.Hk * RT * D;
+  const float* ml = a.part + (size_t)a.max_slots * a.Hk * RT * D;
   const int per = (sp.chunks + kWaves - 1) / kWaves, n0 = wave * per, n1 = min(n0 + per, sp.chunks);
-  const size_t at = ((size_t)it.first_item * a.Hk + hk) * RT + c, step = (size_t)a.Hk * RT;
-  float top = -INFINITY, sum = 0.f;
+  const size_t step = (size_t)a.Hk * RT;
+  for (int e0 = blockIdx.y * kWave; e0 < n_cols * (D / 4); e0 += gridDim.y * kWave) {
+    const int c = (e0 + lane) / (D / 4), d = (e0 + lane - c * (D / 4)) * 4;  // c < RT: RT * D / 4 is a multiple of 64
+    const size_t at = ((size_t)it.slot * a.Hk + hk) * RT + c;
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
-  for (int n = n0; n < n1; ++n) top = fmaxf(top, ml[(at + n * step) * 2]);
-  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    for (int n = n0; n < n1; ++n) top = fmaxf(top, ml[(at + n * step) * 2]);
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int n = n0; n < n1; ++n) {
-    const float mm = ml[(at + n * step) * 2];
-    const float f = mm == -INFINITY ? 0.f : exp2_fast(mm - top);
-    sum += f * ml[(at + n * step) * 2 + 1];
-    o += f * *(const f32x4_t*)(a.part + (at + n * step) * D + d);
-  }
-  part_o[wave][lane] = o;
-  part_m[wave][lane] = top;
-  part_l[wave][lane] = sum;
-  __syncthreads();
-  if (wave != 0 || c >= n_cols) continue;
+    for (int n = n0; n < n1; ++n) {
+      const float mm = ml[(at + n * step) * 2];
+      const float f = mm == -INFINITY ? 0.f : exp2_fast(mm - top);
+      sum += f * ml[(at + n * step) * 2 + 1];
+      o += f * *(const f32x4_t*)(a.part + (at + n * step) * D + d);
+    }
+    __syncthreads();  // the sums of the values before are read
+    part_o[wave][lane] = o;
+    part_m[wave][lane] = top;
+    part_l[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || c >= n_cols) continue;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) top = fmaxf(top, part_m[w][lane]);
-  sum = 0.f;
-  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, part_m[w][lane]);
+    sum = 0.f;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    const float mm = part_m[w][lane], f = mm == -INFINITY ? 0.f : exp2_fast(mm - top);
-    sum += f * part_l[w][lane];
-    o += f * part_o[w][lane];
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int row = r / a.G, head = hk * a.G + (r - row * a.G);
-  uint16_t b[4];
+    for (int w = 0; w < kWaves; ++w) {
+      const float mm = part_m[w][lane], f = mm == -INFINITY ? 0.f : exp2_fast(mm - top);
+      sum += f * part_l[w][lane];
+      o += f * part_o[w][lane];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int r = it.tile * RT + c, row = r / a.G, head = hk * a.G + (r - row * a.G);
+    uint16_t b[4];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) b[x] = Qk<F16>::out(o[x] * inv);
-  *(uint2*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
-      make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+    for (int x = 0; x < 4; ++x) b[x] = Qk<F16>::out(o[x] * inv);
+    *(uint2*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + d) =
+        make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
   }
 }
 
@@ -620,31 +676,46 @@ int col_tiles(int T, int B, int G, int D) {
 }
 
 struct Grid {
-  int ct, target, max_items, max_tiles;
+  int ct, resident, max_tiles, max_slots, groups;
 };
 
-Grid grid_of(int T, int B, int Hq, int Hk, int D) {
+Grid grid_of(int T, int B, int Hq, int Hk, int D, int64_t tokens) {
   const int G = Hq / Hk;
   Grid r;
   r.ct = col_tiles(T, B, G, D);
   const int RT = 16 * r.ct;
   const int64_t cols = (int64_t)T * G;
+  // a request's last tile may be cut: ceil(rows * G / RT) tiles
   r.max_tiles = (int)(cols < cols / RT + B ? cols : cols / RT + B);
-  r.target = (workgroups_per_cu(D, r.ct) * 256 + Hk - 1) / Hk;
-  r.max_items = r.target + r.max_tiles;
+  r.resident = (workgroups_per_cu(D, r.ct) * 256 + Hk - 1) / Hk;
+  // chunk >= total / (kRounds * resident), so the chunks of all tiles are at
+  // most kRounds * resident and one more for each; those of tiles that are cut
+  // (units > chunk) at most twice as many as total / chunk, nor more than the longest table has
+  const int64_t per_tile = (tokens / kUnit + 1 + kMinChunk - 1) / kMinChunk;
+  const int64_t items = kRounds * (int64_t)r.resident + r.max_tiles;
+  const int64_t slots = 2 * kRounds * (int64_t)r.resident;
+  const int64_t most = r.max_tiles * per_tile;
+  r.max_slots = (int)(tokens <= kMinChunk * kUnit ? 0 : most < slots ? most : slots);
+  // Workgroups without an item cost a round of the chip each time it is full of
+  // them (2056 of them 9.6 us beside one request of 1391 tokens), so there are no
+  // more than it holds at a time, or tiles; each takes every so-many-th item.
+  const int64_t wide = r.resident > r.max_tiles ? r.resident : r.max_tiles;
+  r.groups = (int)(most < wide ? most : wide < items ? wide : items);
   return r;
 }
 
 size_t part_bytes(const Grid& gr, int Hk, int D) {
-  return (size_t)gr.max_items * Hk * gr.ct * 16 * (D + 2) * sizeof(float);
+  const size_t n = (size_t)gr.max_slots * Hk * gr.ct * 16 * (D + 2) * sizeof(float);
+  return n ? n : 16;
 }
 
 bool width_ok(int D) { return D == 64 || D == 128 || D == 256 || D == 512; }
 
 template <int D, int CT, bool F16>
 void launch(const AttnArgs& a, const Grid& gr, hipStream_t stream) {
-  hipLaunchKernelGGL((kv_attention_kernel<D, CT, F16>), dim3(gr.max_items * a.Hk), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((kv_attention_kernel<D, CT, F16>), dim3(gr.groups * a.Hk), dim3(kThreads), 0, stream, a);
   // up to 2048 workgroups, each for as many of its tile's values as that leaves
+  if (gr.max_slots == 0) return;
   const int cols = (int)min((int64_t)16 * CT, (int64_t)(a.q_start ? a.T : 1) * a.G), tiles = gr.max_tiles * a.Hk;
   const int parts = min(max(2048 / tiles, 1), (cols * (D / 4) + kWave - 1) / kWave);
   hipLaunchKernelGGL((kv_attention_join_kernel<D, CT, F16>), dim3(tiles, parts), dim3(kThreads), 0, stream, a);
@@ -667,9 +738,9 @@ void launch_d(const AttnArgs& a, const Grid& gr, int D, hipStream_t stream) {
 
 }  // namespace
 
-size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D) {
-  if (T <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || !width_ok(D)) return 0;
-  return part_bytes(grid_of(T, B, Hq, Hk, D), Hk, D);
+size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D, int64_t max_tokens) {
+  if (T <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || !width_ok(D) || max_tokens < 0) return 0;
+  return part_bytes(grid_of(T, B, Hq, Hk, D, max_tokens), Hk, D);
 }
 
 int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, const void* k_cache, const void* v_cache,
@@ -700,13 +771,13 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
     if ((uintptr_t)p & 15) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
   for (const int64_t s : {q_strides[0], q_strides[1], o_strides[0], o_strides[1]})
     if (s % 8) return fail(GI_ERR_INVALID_ARG, "kv_attention: row and head strides must be multiples of 8 elements");
-  const Grid gr = grid_of(T, B, Hq, Hk, D);
-  if ((int64_t)gr.max_items * Hk > 0x7fffffff) return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows");
+  const Grid gr = grid_of(T, B, Hq, Hk, D, (int64_t)max_pages * page_size);
+  if ((int64_t)gr.groups * Hk > 0x7fffffff) return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows");
   if (!workspace || workspace_bytes < part_bytes(gr, Hk, D))
     return fail(GI_ERR_WORKSPACE, "kv_attention: workspace missing or too small");
   AttnArgs a{q, q_strides[0], q_strides[1], (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale,
              block_table, table_stride, seq_lens, q_start, out, o_strides[0], o_strides[1], (float*)workspace,
-             num_pages, scale * kLog2e, T, B, Hk, Hq / Hk, max_pages, lp, window, gr.target, gr.max_items};
+             num_pages, scale * kLog2e, T, B, Hk, Hq / Hk, max_pages, lp, window, gr.resident, gr.max_slots};
   if (dtype == GI_DTYPE_FP16) launch_d<true>(a, gr, D, stream);
   else launch_d<false>(a, gr, D, stream);
   return after_launch("kv_attention launch");

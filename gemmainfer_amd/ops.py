@@ -860,7 +860,7 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
         q = q.clone(memory_format=torch.contiguous_format)
     qs = q.stride()
     lib = L.load()
-    nbytes = lib.gi_kv_attention_workspace_bytes(t, b, hq, hk, d)
+    nbytes = lib.gi_kv_attention_workspace_bytes(t, b, hq, hk, d, cols * page)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with _launch_on(dev):
         L.check(lib.gi_kv_attention(

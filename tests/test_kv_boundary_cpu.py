@@ -91,7 +91,7 @@ ATTN = dict(q=VP, dtype=L.DTYPE_BF16, a=256, b=64, kc=VP, vc=VP, ks=VP, vs=VP, t
 
 @pytest.mark.parametrize("over,code,frag", [
     (dict(), L.GI_ERR_WORKSPACE, "workspace"),
-    (dict(ws=VP, wsb=1024), L.GI_ERR_WORKSPACE, "workspace"),
+    (dict(cols=400, stride=400, ws=VP, wsb=1024), L.GI_ERR_WORKSPACE, "workspace"),
     (dict(dtype=L.DTYPE_FP32), L.GI_ERR_UNSUPPORTED, "bf16 or fp16"),
     (dict(Hq=5), L.GI_ERR_INVALID_ARG, "multiple of Hk"),
     (dict(D=96), L.GI_ERR_UNSUPPORTED, "64, 128, 256 and 512"),
@@ -114,9 +114,11 @@ def test_kv_attention_refuses(lib, over, code, frag):
 
 def test_workspace_query_is_host_only(lib):
     q = lib.gi_kv_attention_workspace_bytes
-    assert q(0, 1, 16, 8, 256) == 0 and q(1, 0, 16, 8, 256) == 0 and q(1, 1, 15, 8, 256) == 0 and q(1, 1, 16, 8, 96) == 0
-    assert 0 < q(1, 1, 16, 8, 256) < 1 << 24
-    assert q(64, 64, 16, 8, 256) < 1 << 26
+    for bad in ((0, 1, 16, 8, 256), (1, 0, 16, 8, 256), (1, 1, 15, 8, 256), (1, 1, 16, 8, 96)):
+        assert q(*bad, 4096) == 0
+    assert 0 < q(1, 1, 16, 8, 256, 256) < 64          # one chunk: nothing to join
+    assert q(1, 1, 16, 8, 256, 4096) < 1 << 24
+    assert q(64, 64, 16, 8, 256, 1 << 20) < 1 << 27    # bounded by what the chip holds, not by the lengths
 
 
 def test_device_calls_reject_host_tensors():
