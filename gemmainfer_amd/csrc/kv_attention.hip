@@ -31,10 +31,12 @@ constexpr int kRounds = 4;
 // what a compute unit holds of a kernel: by its registers, two waves a SIMD or one
 constexpr int workgroups_per_cu(int D, int CT) { return D * CT <= (CT == 1 ? 256 : 128) ? 2 : 1; }
 constexpr float kLog2e = 1.4426950408889634f;
-// Weights go to the matrix cores in fp16 as 2^(t - m + kBias), at most 2^(kBias
-// + kSlack): fp16 is normal down to 2^-14, so a weight 2^-21 of the largest
-// still has all 11 bits.
-constexpr float kBias = 7.f, kSlack = 8.f;
+// Weights go to the matrix cores in fp16 as 2^(t - m + kBias).  The reference m
+// is a maximum of earlier rows and follows when a lane's 16 weights sum to more than
+// kMostSum, so none is over 2^15; fp16 is normal down to 2^-14, so a weight
+// 2^-21 of that of m still has all 11 bits.
+constexpr float kBias = 7.f;
+constexpr float kMostSum = 32768.f;
 
 struct AttnArgs {
   const void* q;
@@ -300,10 +302,11 @@ struct UnitRef {
 //
 // V's scale joins the exponent: t = s + log2(vs), weights 2^(t - m), m over t.
 // The sum of softmax weights is then sum 2^(t - m) / vs.  With it the weights
-// of V's codes never exceed 2^(kBias + kSlack) whatever the scales are, and the
-// maximum is over what each row can contribute.  m follows the true maximum
-// only when it is kSlack behind: the sums are scaled anew a few times a call,
-// not once a unit.
+// of V's codes stay in fp16's range whatever the scales are, and the
+// maximum is over what each row can contribute.  Most units need no maximum at
+// all: their weights are formed with the reference there is, and only where a sum
+// shows that one has grown too large are the maximum found, the sums scaled and the weights
+// formed again.
 template <int D, int CT, bool F16>
 __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attention_kernel(AttnArgs a) {
   constexpr int RT = 16 * CT;
@@ -360,11 +363,10 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
   if (kQLds) __syncthreads();
 
   f32x4_t acc[CT][DT];
-  float m[CT], mref[CT], l[CT];
+  float m[CT], l[CT];  // the reference of the weights (-inf: none yet), their sum over v's scale
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     m[ct] = -INFINITY;
-    mref[ct] = 0.f;
     l[ct] = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[ct][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -419,113 +421,120 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
       const bool edge = tok + kUnit - 1 > pos_min || (a.window > 0 && tok <= pos_max - a.window);
       f32x4_t s[CT][4];
       f16x8_t p[CT][2];
-      uint32_t keep[4];
+      auto ahead = [&](int st) {
+        if (st + kRing - 1 < kSteps) issue(cur, st + kRing - 1);
+        else issue(nxt, st + kRing - 1 - kSteps);
+        __builtin_amdgcn_sched_barrier(kFree);
+      };
+
+      // ---- scores
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[ct][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int st = 0; st < kSteps; ++st) {
-        if (st + kRing - 1 < kSteps) issue(cur, st + kRing - 1);
-        else issue(nxt, st + kRing - 1 - kSteps);
-        __builtin_amdgcn_sched_barrier(kFree);
-        if (st < KS) {
-          // ---- scores, 64 dimensions
-          frag k[4][2];
+      for (int st = 0; st < KS; ++st) {
+        ahead(st);
+        frag k[4][2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint4 w = ring[st % kRing][j];
-            k[j][0] = Qk<F16>::codes(w.x, w.y);
-            k[j][1] = Qk<F16>::codes(w.z, w.w);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-              const frag q = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * st + h) * kWave + lane])
-                                   : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * st + h];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) s[ct][j] = Qk<F16>::mfma(k[j][h], q, s[ct][j]);
-            }
+        for (int j = 0; j < 4; ++j) {
+          const uint4 w = ring[st % kRing][j];
+          k[j][0] = Qk<F16>::codes(w.x, w.y);
+          k[j][1] = Qk<F16>::codes(w.z, w.w);
         }
-        if (st == KS - 1) {
-          // ---- weights
-          const float cs = cur.ks * a.scale, cv = __log2f(cur.vs), inv_vs = 1.f / cur.vs;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
+            const frag q = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * st + h) * kWave + lane])
+                                 : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * st + h];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) s[ct][j][r] = fmaf(s[ct][j][r], cs, cv);
-            if (edge) {
-              const int hi = hi_pos[ct] - (tok + 16 * g), lo = a.window > 0 ? hi - a.window : -1;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  s[ct][j][r] = 4 * j + r <= hi && 4 * j + r > lo ? s[ct][j][r] : -INFINITY;
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) top = fmaxf(top, s[ct][j][r]);
-            top = column_max(top);
-            if (__any(top > m[ct] + kSlack)) {
-              const float now = fmaxf(m[ct], top);
-              const float next = now == -INFINITY ? 0.f : now;
-              const float f = m[ct] == -INFINITY ? 0.f : exp2_fast(mref[ct] - next);  // -inf: nothing was added yet
-              m[ct] = now;
-              mref[ct] = next;
-              l[ct] *= f;
-#pragma unroll
-              for (int dt = 0; dt < DT; ++dt) acc[ct][dt] *= f;
-            }
-            const float shift = kBias - mref[ct];
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float w = exp2_fast(s[ct][j][r] + shift);
-                sum += w;
-                p[ct][j >> 1][(j & 1) * 4 + r] = (_Float16)w;
-              }
-            // rows that are not seen weigh nothing, whatever their page's scale is
-            l[ct] += sum == 0.f ? 0.f : sum * inv_vs;
+            for (int j = 0; j < 4; ++j) s[ct][j] = Qk<F16>::mfma(k[j][h], q, s[ct][j]);
           }
-          // rows of V that no column sees may hold anything
-          const int last = min(pos_max - (tok + 16 * g), 15);
-          const int first = a.window > 0 ? pos_min - a.window + 1 - (tok + 16 * g) : 0;
+      }
+
+      // ---- weights
+      float c1 = cur.ks * a.scale, c0 = __log2f(cur.vs);
+      const float inv_vs = 1.f / cur.vs;
+      if (edge) {
+        // what is not seen scores -inf, whatever its page's scale is
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            keep[x] = 0;
-            if (edge) {
+        for (int ct = 0; ct < CT; ++ct) {
+          const int hi = hi_pos[ct] - (tok + 16 * g), lo = a.window > 0 ? hi - a.window : -1;
 #pragma unroll
-              for (int y = 0; y < 4; ++y)
-                if (4 * x + y <= last && 4 * x + y >= first) keep[x] |= 0xffu << (8 * y);
-            }
-          }
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              s[ct][j][r] = 4 * j + r <= hi && 4 * j + r > lo ? fmaf(s[ct][j][r], c1, c0) : -INFINITY;
         }
-        if (st >= KS) {
-          // ---- O^T += V^T P^T, 64 dimensions
-          if (edge) {
+        c1 = 1.f;
+        c0 = 0.f;
+      }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint4& w = ring[st % kRing][i];
-              w = make_uint4(w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]);
+      for (int ct = 0; ct < CT; ++ct) {
+        auto weigh = [&]() {
+          const float shift = c0 + (kBias - (m[ct] == -INFINITY ? 0.f : m[ct]));
+          float sum = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float w = exp2_fast(fmaf(s[ct][j][r], c1, shift));
+              sum += w;
+              p[ct][j >> 1][(j & 1) * 4 + r] = (_Float16)w;
             }
+          return sum;
+        };
+        float sum = weigh();
+        // the reference has to follow: a weight is near what fp16 holds, or there is none yet
+        if (__any(!(sum <= kMostSum) || m[ct] == -INFINITY)) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, fmaf(s[ct][j][r], c1, c0));
+          top = fmaxf(m[ct], column_max(top));
+          if (m[ct] != -INFINITY) {
+            const float f = exp2_fast(m[ct] - top);
+            l[ct] *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[ct][dt] *= f;
           }
+          m[ct] = top;
+          sum = weigh();
+        }
+        // rows that are not seen weigh nothing, whatever their page's scale is
+        l[ct] += sum == 0.f ? 0.f : sum * inv_vs;
+      }
+
+      // ---- O^T += V^T P^T
+      // (masked in every unit: one straight line of code is scheduled better than two, 3% of the
+      // instructions of 64 columns)
+      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+      if (edge) {  // rows that no column sees may hold anything
+        const int last = min(pos_max - (tok + 16 * g), 15);
+        const int first = a.window > 0 ? pos_min - a.window + 1 - (tok + 16 * g) : 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 w = ring[st % kRing][i];
-            const f16x8_t v0 = codes_f16(w.x, w.y), v1 = codes_f16(w.z, w.w);
-            const int dt = (st - KS) * 4 + i;
+        for (int x = 0; x < 4; ++x) {
+          keep[x] = 0;
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) acc[ct][dt] = mfma_f16(v0, p[ct][0], acc[ct][dt]);
+          for (int y = 0; y < 4; ++y)
+            if (4 * x + y <= last && 4 * x + y >= first) keep[x] |= 0xffu << (8 * y);
+        }
+      }
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) acc[ct][dt] = mfma_f16(v1, p[ct][1], acc[ct][dt]);
-          }
+      for (int st = KS; st < kSteps; ++st) {
+        ahead(st);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint4 w = ring[st % kRing][i];
+          w = make_uint4(w.x & keep[0], w.y & keep[1], w.z & keep[2], w.w & keep[3]);
+          const f16x8_t v0 = codes_f16(w.x, w.y), v1 = codes_f16(w.z, w.w);
+          const int dt = (st - KS) * 4 + i;
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[ct][dt] = mfma_f16(v0, p[ct][0], acc[ct][dt]);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) acc[ct][dt] = mfma_f16(v1, p[ct][1], acc[ct][dt]);
         }
       }
       cur = nxt;
@@ -539,7 +548,7 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
     l[ct] += __shfl_xor(l[ct], 16, kWave);
     l[ct] += __shfl_xor(l[ct], 32, kWave);
     if (g == 0) {
-      red_m[wave][ct * 16 + i16] = m[ct] == -INFINITY ? -INFINITY : mref[ct];
+      red_m[wave][ct * 16 + i16] = m[ct];
       red_l[wave][ct * 16 + i16] = l[ct];
     }
   }
@@ -550,7 +559,7 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, red_m[w][ct * 16 + i16]);
-    f[ct] = m[ct] == -INFINITY ? 0.f : exp2_fast(mref[ct] - top);
+    f[ct] = m[ct] == -INFINITY ? 0.f : exp2_fast(m[ct] - top);
     if (m[ct] == -INFINITY && l[ct] != l[ct]) f[ct] = l[ct];  // only scores without a value: they stay NaN
   }
 #pragma unroll
