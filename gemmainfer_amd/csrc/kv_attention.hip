@@ -34,8 +34,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Weights go to the matrix cores in fp16 as 2^(t - m + kBias).  The reference m
 // is a maximum of earlier rows and follows when a lane's 16 weights sum to more than
 // kMostSum, so none is over 2^15; fp16 is normal down to 2^-14, so a weight
-// 2^-21 of that of m still has all 11 bits.
-constexpr float kBias = 7.f;
+// 2^-17 of that of m still has all 11 bits, and a lighter one is off by at most 2^-28 of it.
+constexpr float kBias = 3.f;
 constexpr float kMostSum = 32768.f;
 
 struct AttnArgs {
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
     for (int s = 0; s < 2 * KS; ++s) {
       if (kQLds && (ct * 2 * KS + s) % kWaves != wave) continue;
       const uint4 w = *(const uint4*)(src + (s >> 1) * 64 + g * 16 + (s & 1) * 8);
-      if (kQLds) q_lds[(ct * 2 * KS + s) * kWave + lane] = w;
+      if (kQLds) q_lds[(s * CT + ct) * kWave + lane] = w;
       else qf[kQLds ? 0 : ct][kQLds ? 0 : s] = __builtin_bit_cast(frag, w);
     }
   }
@@ -432,6 +432,11 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[ct][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      uint4 q_next[3];
+      if (kQLds) {
+        q_next[0] = q_lds[lane];
+        q_next[1] = q_lds[kWave + lane];
+      }
 #pragma unroll
       for (int st = 0; st < KS; ++st) {
         ahead(st);
@@ -446,7 +451,12 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int ct = 0; ct < CT; ++ct) {
-            const frag q = kQLds ? __builtin_bit_cast(frag, q_lds[(ct * 2 * KS + 2 * st + h) * kWave + lane])
+            if (kQLds) {  // two operands ahead of the products: LDS takes as long as eight of them
+              const int n = (2 * st + h) * CT + ct;
+              if (n + 2 < 2 * KS * CT) q_next[(n + 2) % 3] = q_lds[(n + 2) * kWave + lane];
+              __builtin_amdgcn_sched_barrier(0x16);
+            }
+            const frag q = kQLds ? __builtin_bit_cast(frag, q_next[((2 * st + h) * CT + ct) % 3])
                                  : qf[kQLds ? 0 : ct][kQLds ? 0 : 2 * st + h];
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[ct][j] = Qk<F16>::mfma(k[j][h], q, s[ct][j]);
