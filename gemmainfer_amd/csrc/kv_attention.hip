@@ -51,6 +51,7 @@ struct AttnArgs {
   const int32_t* q_start;  // null: one row a request
   void* out;
   int64_t o_st, o_sh;
+  int* chunk;              // what the join has to know, in front of
   float* part;             // [max_slots * Hk][RT][D] partial sums, then [max_slots * Hk][RT] (maximum, sum)
   int64_t num_pages;
   float scale;             // with log2(e)
@@ -107,54 +108,59 @@ __device__ __forceinline__ Load load_of(const AttnArgs& a, int b) {
   return r;
 }
 
-__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const int u = __shfl_up(v, off, kWave);
-    if (lane >= off) v += u;
-  }
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 
-template <typename N>
-__device__ __forceinline__ N wave_sum(N v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
-  return v;
+// ceil(n / d), n + d at most 2^25: a quotient in fp32 is off by one at most.
+__device__ __forceinline__ int ceil_div(int n, int d) {
+  n += d - 1;
+  int q = (int)((float)n * __builtin_amdgcn_rcpf((float)d));
+  const int r = n - q * d;
+  q += r >= d ? 1 : 0;
+  return r < 0 ? q - 1 : q;
 }
 
-// The chunk, in units: `total` tile units of a kv head go to `resident`
-// workgroups that the chip holds at a time, in k = 1 ... 4 rounds.  One round
+// The chunk, in units: the tile units of a kv head go to `resident` workgroups
+// that the chip holds at a time, in k = 1 ... 4 rounds.  One round
 // is best where the chunks come out even (a few long requests: two of 70001 and 130005
 // tokens 77 us in one round, 91 in two), several where many requests of
 // other lengths leave workgroups idle (47 up to 8190 tokens: 214, 202 and 194 us in one,
 // two and three).  k is the one with the least estimate: rounds of whole
 // chunks, or what any order of work stays under, and two units to start each round.
+// Every workgroup finds the same (the join takes it from the first one).
 template <int RT>
 __device__ __forceinline__ int chunk_of(const AttnArgs& a) {
   const int lane = threadIdx.x & 63;
   const Load head = load_of<RT>(a, lane);
-  double total = 0.;
+  float total = 0.f;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
     const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
-    total += (double)l.tiles * l.units;
+    total += (float)l.tiles * (float)l.units;
   }
-  total = wave_sum(total);
+  // not less than the exact total, whatever was rounded: chunk >= total / (k * resident)
+  const float each = wave_sum_f32(total) * 1.0001f * __builtin_amdgcn_rcpf((float)a.resident);
   int best = 0;
   float least = 0.f;
 #pragma unroll 1
   for (int k = 1; k <= kRounds; ++k) {
-    int c = (int)(total / ((double)a.resident * k)) + 1;
+    // a chunk of 2^24 units holds any request
+    int c = (int)fminf(each * __builtin_amdgcn_rcpf((float)k), 16777200.f) + 1;
     c = (max(c, kMinChunk) + kWaves - 1) / kWaves * kWaves;
     if (k > 1 && c >= best) break;
-    int items = 0;
+    float items = 0.f;
     for (int b0 = 0; b0 < a.B; b0 += kWave) {
       const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
-      items += l.tiles * ((l.units + c - 1) / c);
+      items += (float)l.tiles * (float)ceil_div(l.units, c);
     }
-    items = wave_sum(items);
-    const int rounds = (items + a.resident - 1) / a.resident;
-    const float cost = fminf((float)rounds * c, (float)(total / a.resident) + c) + 2.f * rounds;
+    const float rounds = ceilf(wave_sum_f32(items) * __builtin_amdgcn_rcpf((float)a.resident));
+    const float cost = fminf(rounds * c, each + c) + 2.f * rounds;
     if (k == 1 || cost < least) {
       best = c;
       least = cost;
@@ -171,10 +177,10 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int chunk, int want
   int items = 0, tiles = 0, slots = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
     const Load l = load_of<RT>(a, b0 + lane);
-    const int chunks = max((l.units + chunk - 1) / chunk, 1);
+    const int chunks = max(ceil_div(l.units, chunk), 1);
     const int n = l.tiles * chunks, n_slots = chunks > 1 ? n : 0;
     const int count = by_tile ? l.tiles : n;
-    const int end = (by_tile ? tiles : items) + wave_scan(count, lane), slot_end = slots + wave_scan(n_slots, lane);
+    const int end = (by_tile ? tiles : items) + wave_scan(count), slot_end = slots + wave_scan(n_slots);
     const unsigned long long hit = __ballot(want >= end - count && want < end);
     if (hit) {
       const int src = __ffsll(hit) - 1;
@@ -214,7 +220,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Item& it) {
   s.lo = 0;
   if (a.window > 0) s.lo = max(s.pos_min - a.window + 1, 0) / kUnit;
   s.hi = s.pos_max < 0 ? 0 : s.pos_max / kUnit + 1;
-  s.chunks = max((s.hi - s.lo + it.chunk - 1) / it.chunk, 1);
+  s.chunks = max(ceil_div(s.hi - s.lo, it.chunk), 1);
   return s;
 }
 
@@ -332,6 +338,7 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
   const int wave = uniform(threadIdx.x >> 6);
   const int hk = blockIdx.x % a.Hk;
   const int chunk = chunk_of<RT>(a);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.chunk = chunk;
   Item it;
   for (int want = blockIdx.x / a.Hk; find_item<RT>(a, chunk, want, false, it); want += gridDim.x / a.Hk) {
   const Span sp = span_of<RT>(a, it);
@@ -632,7 +639,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_join_kernel(AttnArgs a)
   __shared__ f32x4_t part_o[kWaves][kWave];
   __shared__ float part_m[kWaves][kWave], part_l[kWaves][kWave];
   const int hk = blockIdx.x % a.Hk;
-  const int chunk = chunk_of<RT>(a);
+  const int chunk = *a.chunk;
   Item it;
   if (!find_item<RT>(a, chunk, blockIdx.x / a.Hk, true, it)) return;
   const Span sp = span_of<RT>(a, it);
@@ -723,9 +730,10 @@ Grid grid_of(int T, int B, int Hq, int Hk, int D, int64_t tokens) {
   return r;
 }
 
+constexpr size_t kHeader = 64;  // bytes of the workspace in front of the partial sums
+
 size_t part_bytes(const Grid& gr, int Hk, int D) {
-  const size_t n = (size_t)gr.max_slots * Hk * gr.ct * 16 * (D + 2) * sizeof(float);
-  return n ? n : 16;
+  return kHeader + (size_t)gr.max_slots * Hk * gr.ct * 16 * (D + 2) * sizeof(float);
 }
 
 bool width_ok(int D) { return D == 64 || D == 128 || D == 256 || D == 512; }
@@ -795,7 +803,8 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
   if (!workspace || workspace_bytes < part_bytes(gr, Hk, D))
     return fail(GI_ERR_WORKSPACE, "kv_attention: workspace missing or too small");
   AttnArgs a{q, q_strides[0], q_strides[1], (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale,
-             block_table, table_stride, seq_lens, q_start, out, o_strides[0], o_strides[1], (float*)workspace,
+             block_table, table_stride, seq_lens, q_start, out, o_strides[0], o_strides[1], (int*)workspace,
+             (float*)((char*)workspace + kHeader),
              num_pages, scale * kLog2e, T, B, Hk, Hq / Hk, max_pages, lp, window, gr.resident, gr.max_slots};
   if (dtype == GI_DTYPE_FP16) launch_d<true>(a, gr, D, stream);
   else launch_d<false>(a, gr, D, stream);
