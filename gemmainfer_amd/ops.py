@@ -21,7 +21,6 @@ kv_attention.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 import threading
@@ -62,9 +61,9 @@ def _require(cond: bool, msg: str, exc=ValueError) -> None:
 def _on_device(*tensors: torch.Tensor) -> torch.device:
     dev = tensors[0].device
     for t in tensors:
-        if not t.is_cuda:
-            raise TypeError("gemmainfer_amd ops take ROCm device tensors only")
-        if t.device != dev:
+        if t.device != dev or not t.is_cuda:
+            if not all(u.is_cuda for u in tensors):
+                raise TypeError("gemmainfer_amd ops take ROCm device tensors only")
             raise ValueError(f"all tensors must be on {dev}, got {t.device}")
     return dev
 
@@ -593,12 +592,16 @@ _ROW_DTYPES = (torch.bfloat16, torch.float16)
 
 # A decode step calls these a few times a layer with kernels of microseconds:
 # messages are only formatted where they are raised.
-def _launch_on(device: torch.device):
-    """Kernels are launched on the current device: make it the tensors' own."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-_HERE = contextlib.nullcontext()
+def _launch(device: torch.device, what: str, *args) -> None:
+    """gi_``what``(*args, stream).  Kernels are launched on the current device: make it the tensors' own."""
+    fn = getattr(L.load(), "gi_" + what)
+    if torch.cuda.current_device() == device.index:
+        st = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, _stream(device))
+    if st != L.GI_OK:
+        L.check(st, what)
 
 
 def kv_cache(num_pages: int, kv_heads: int, page_size: int, head_dim: int, device="cuda") -> KVCache:
@@ -680,11 +683,10 @@ def kv_slots(ctx_lens, new_lens, block_table, free_pages, free_used, page_size, 
     cols, stride = _table(block_table, b, "kv_slots")
     slots, positions = torch.empty((2, num_rows), dtype=torch.int64, device=dev).unbind(0)
     q_start, seq_lens, status = torch.empty(2 * b + 4, dtype=torch.int32, device=dev).split((b + 1, b, 3))
-    with _launch_on(dev):
-        L.check(L.load().gi_kv_slots(
-            ctx_lens.data_ptr(), new_lens.data_ptr(), b, block_table.data_ptr(), cols, stride, free_pages.data_ptr(),
-            free_pages.numel(), free_used.data_ptr(), page_size, slots.data_ptr(), positions.data_ptr(), num_rows,
-            q_start.data_ptr(), seq_lens.data_ptr(), status.data_ptr(), _stream(dev)), "kv_slots")
+    _launch(dev, "kv_slots",
+        ctx_lens.data_ptr(), new_lens.data_ptr(), b, block_table.data_ptr(), cols, stride, free_pages.data_ptr(),
+        free_pages.numel(), free_used.data_ptr(), page_size, slots.data_ptr(), positions.data_ptr(), num_rows,
+        q_start.data_ptr(), seq_lens.data_ptr(), status.data_ptr())
     return KVSlots(slots, positions, q_start, seq_lens, status)
 
 
@@ -760,11 +762,10 @@ def rope_rows(q, k, positions, inv_freq, *, interleaved: bool = False, mscale: f
         kos = (hk * d, d)
     if t == 0:
         return qo, ko
-    with _launch_on(dev):
-        L.check(L.load().gi_rope_rows(
-            q.data_ptr(), qo.data_ptr(), None if k is None else k.data_ptr(), None if k is None else ko.data_ptr(),
-            positions.data_ptr(), inv_freq.data_ptr(), _DTYPE_CODE[q.dtype], t, hq, hk, d, rot, bool(interleaved),
-            mscale, qs[0], qs[1], qos[0], qos[1], ks[0], ks[1], kos[0], kos[1], _stream(dev)), "rope_rows")
+    _launch(dev, "rope_rows",
+        q.data_ptr(), qo.data_ptr(), None if k is None else k.data_ptr(), None if k is None else ko.data_ptr(),
+        positions.data_ptr(), inv_freq.data_ptr(), _DTYPE_CODE[q.dtype], t, hq, hk, d, rot, bool(interleaved),
+        mscale, qs[0], qs[1], qos[0], qos[1], ks[0], ks[1], kos[0], kos[1])
     return qo, ko
 
 
@@ -790,11 +791,9 @@ def kv_append(k, v, slots, cache: KVCache) -> None:
     if ks[2] != 1 or vs[2] != 1:
         raise ValueError("kv_append: the last dimension of k and v must be contiguous")
     _vector(slots, torch.int64, "kv_append", "slots")
-    with _launch_on(dev):
-        L.check(L.load().gi_kv_append(
-            k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), t, hk, d,
-            page, pages, cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr(),
-            _stream(dev)), "kv_append")
+    _launch(dev, "kv_append",
+        k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), t, hk, d,
+        page, pages, cache[0].data_ptr(), cache[1].data_ptr(), cache[2].data_ptr(), cache[3].data_ptr())
 
 
 def _rows_aligned(x):
@@ -862,11 +861,9 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
     lib = L.load()
     nbytes = lib.gi_kv_attention_workspace_bytes(t, b, hq, hk, d, cols * page)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _launch_on(dev):
-        L.check(lib.gi_kv_attention(
-            q.data_ptr(), _DTYPE_CODE[q.dtype], qs[0], qs[1], cache[0].data_ptr(), cache[1].data_ptr(),
-            cache[2].data_ptr(), cache[3].data_ptr(), block_table.data_ptr(), cols, stride, seq_lens.data_ptr(),
-            None if q_start is None else q_start.data_ptr(), out.data_ptr(), os[0], os[1], t, b, hq, hk, d, page,
-            pages, d ** -0.5 if scale is None else scale, window, ws.data_ptr(), nbytes, _stream(dev)),
-            "kv_attention")
+    _launch(dev, "kv_attention",
+        q.data_ptr(), _DTYPE_CODE[q.dtype], qs[0], qs[1], cache[0].data_ptr(), cache[1].data_ptr(),
+        cache[2].data_ptr(), cache[3].data_ptr(), block_table.data_ptr(), cols, stride, seq_lens.data_ptr(),
+        None if q_start is None else q_start.data_ptr(), out.data_ptr(), os[0], os[1], t, b, hq, hk, d, page,
+        pages, d ** -0.5 if scale is None else scale, window, ws.data_ptr(), nbytes)
     return out
