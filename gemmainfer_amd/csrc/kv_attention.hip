@@ -28,6 +28,7 @@ constexpr int kThreads = kWaves * kWave;
 constexpr int kUnit = 64;      // cache rows a wave takes at a time
 constexpr int kMinChunk = 4;   // units: one a wave
 constexpr int kRounds = 4;
+constexpr int kEnds = 64;      // bytes of the plan in front of the running counts
 // what a compute unit holds of a kernel: by its registers, two waves a SIMD or one
 constexpr int workgroups_per_cu(int D, int CT) { return D * CT <= (CT == 1 ? 256 : 128) ? 2 : 1; }
 constexpr float kLog2e = 1.4426950408889634f;
@@ -51,7 +52,7 @@ struct AttnArgs {
   const int32_t* q_start;  // null: one row a request
   void* out;
   int64_t o_st, o_sh;
-  int* chunk;              // what the join has to know, in front of
+  int* plan;               // the chunk; at kEnds bytes, for more than 64 requests, int4 [B] running counts
   float* part;             // [max_slots * Hk][RT][D] partial sums, then [max_slots * Hk][RT] (maximum, sum)
   int64_t num_pages;
   float scale;             // with log2(e)
@@ -67,7 +68,9 @@ struct AttnArgs {
 // finds its own from the request lengths, on the device, so the launch needs no
 // host copy of them and can be replayed from a graph for other lengths.  The
 // chunk is the same for all requests: a long one is shared by as many
-// workgroups as a batch of short ones.
+// workgroups as a batch of short ones.  Up to 64 requests are one load of a
+// wave; for more, a workgroup launched first writes the chunk and running counts of
+// items, tiles and partial sums, and the others search those.
 struct Item {
   int b, tile, chunk_no, chunk, q0, rows, len;
   int slot;   // of the tile's first partial sum, among those of one kv head
@@ -104,7 +107,7 @@ __device__ __forceinline__ Load load_of(const AttnArgs& a, int b) {
   r.len = min(len, cap);
   r.tiles = (r.rows * a.G + RT - 1) / RT;  // rows * G at most 2^30
   r.units = (r.len + kUnit - 1) / kUnit;
-  if (a.window > 0 && a.window <= cap) r.units = min(r.units, (a.window + RT) / kUnit + 2);
+  if (a.window > 0) r.units = min(r.units, (a.window + RT) / kUnit + 2);  // a window is shorter than the table
   return r;
 }
 
@@ -134,18 +137,12 @@ __device__ __forceinline__ int ceil_div(int n, int d) {
 // other lengths leave workgroups idle (47 up to 8190 tokens: 214, 202 and 194 us in one,
 // two and three).  k is the one with the least estimate: rounds of whole
 // chunks, or what any order of work stays under, and two units to start each round.
-// Every workgroup finds the same (the join takes it from the first one).
-template <int RT>
-__device__ __forceinline__ int chunk_of(const AttnArgs& a) {
-  const int lane = threadIdx.x & 63;
-  const Load head = load_of<RT>(a, lane);
-  float total = 0.f;
-  for (int b0 = 0; b0 < a.B; b0 += kWave) {
-    const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
-    total += (float)l.tiles * (float)l.units;
-  }
+// `sum` adds a number of each request up.
+template <typename Sum>
+__device__ __forceinline__ int choose_chunk(const AttnArgs& a, Sum&& sum) {
+  const float total = sum([](const Load& l) { return (float)l.tiles * (float)l.units; });
   // not less than the exact total, whatever was rounded: chunk >= total / (k * resident)
-  const float each = wave_sum_f32(total) * 1.0001f * __builtin_amdgcn_rcpf((float)a.resident);
+  const float each = total * 1.0001f * __builtin_amdgcn_rcpf((float)a.resident);
   int best = 0;
   float least = 0.f;
 #pragma unroll 1
@@ -154,12 +151,8 @@ __device__ __forceinline__ int chunk_of(const AttnArgs& a) {
     int c = (int)fminf(each * __builtin_amdgcn_rcpf((float)k), 16777200.f) + 1;
     c = (max(c, kMinChunk) + kWaves - 1) / kWaves * kWaves;
     if (k > 1 && c >= best) break;
-    float items = 0.f;
-    for (int b0 = 0; b0 < a.B; b0 += kWave) {
-      const Load l = b0 == 0 ? head : load_of<RT>(a, b0 + lane);
-      items += (float)l.tiles * (float)ceil_div(l.units, c);
-    }
-    const float rounds = ceilf(wave_sum_f32(items) * __builtin_amdgcn_rcpf((float)a.resident));
+    const float items = sum([c](const Load& l) { return (float)l.tiles * (float)ceil_div(l.units, c); });
+    const float rounds = ceilf(items * __builtin_amdgcn_rcpf((float)a.resident));
     const float cost = fminf(rounds * c, each + c) + 2.f * rounds;
     if (k == 1 || cost < least) {
       best = c;
@@ -170,39 +163,111 @@ __device__ __forceinline__ int chunk_of(const AttnArgs& a) {
   return __builtin_amdgcn_readfirstlane(best);
 }
 
+struct Counts {
+  int items, tiles, slots;
+};
+
+__device__ __forceinline__ Counts counts_of(const Load& l, int chunk) {
+  const int chunks = max(ceil_div(l.units, chunk), 1), n = l.tiles * chunks;
+  return Counts{n, l.tiles, chunks > 1 ? n : 0};
+}
+
+// The chunk of up to 64 requests: every workgroup finds the same.
+template <int RT>
+__device__ __forceinline__ int chunk_of_few(const AttnArgs& a) {
+  const Load mine = load_of<RT>(a, threadIdx.x & 63);
+  return choose_chunk(a, [&](auto&& number) { return wave_sum_f32(number(mine)); });
+}
+
+// The plan of more: one workgroup.
+constexpr int kPlanThreads = 1024;
+template <int RT>
+__global__ __launch_bounds__(kPlanThreads) void kv_attention_plan_kernel(AttnArgs a) {
+  __shared__ float part[kPlanThreads / kWave];
+  __shared__ int sums[3][kPlanThreads / kWave];
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const int chunk = choose_chunk(a, [&](auto&& number) {
+    float v = 0.f;
+    for (int b = tid; b < a.B; b += kPlanThreads) v += number(load_of<RT>(a, b));
+    v = wave_sum_f32(v);
+    __syncthreads();  // the sum before is read
+    if ((tid & 63) == 0) part[wave] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int w = 0; w < kPlanThreads / kWave; ++w) v += part[w];
+    return v;
+  });
+  if (tid == 0) *a.plan = chunk;
+  int4* ends = (int4*)((char*)a.plan + kEnds);
+  int carry[3] = {0, 0, 0};
+  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+    const Counts c = counts_of(load_of<RT>(a, b0 + tid), chunk);
+    int v[3] = {wave_scan(c.items), wave_scan(c.tiles), wave_scan(c.slots)};
+    __syncthreads();
+    if ((tid & 63) == 63)
+      for (int x = 0; x < 3; ++x) sums[x][wave] = v[x];
+    __syncthreads();
+    for (int x = 0; x < 3; ++x) {
+      int all = 0;
+      for (int w = 0; w < kPlanThreads / kWave; ++w) {
+        if (w == wave) v[x] += carry[x] + all;
+        all += sums[x][w];
+      }
+      carry[x] += all;
+    }
+    if (b0 + tid < a.B) ends[b0 + tid] = make_int4(v[0], v[1], v[2], 0);
+  }
+}
+
 // Item `want` of the list (by_tile: the first item of tile `want`); false past its end.
 template <int RT>
 __device__ __forceinline__ bool find_item(const AttnArgs& a, int chunk, int want, bool by_tile, Item& it) {
   const int lane = this_lane();
-  int items = 0, tiles = 0, slots = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kWave) {
-    const Load l = load_of<RT>(a, b0 + lane);
-    const int chunks = max(ceil_div(l.units, chunk), 1);
-    const int n = l.tiles * chunks, n_slots = chunks > 1 ? n : 0;
-    const int count = by_tile ? l.tiles : n;
-    const int end = (by_tile ? tiles : items) + wave_scan(count), slot_end = slots + wave_scan(n_slots);
+  int in, slot;
+  Load l;
+  if (a.B <= kWave) {
+    const Load mine = load_of<RT>(a, lane);
+    const Counts c = counts_of(mine, chunk);
+    const int count = by_tile ? c.tiles : c.items;
+    const int end = wave_scan(count), slot_end = wave_scan(c.slots);
     const unsigned long long hit = __ballot(want >= end - count && want < end);
-    if (hit) {
-      const int src = __ffsll(hit) - 1;
-      auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
-      const int in = want - pick(end - count), per = pick(chunks);
-      it.b = b0 + src;
-      it.tile = by_tile ? in : in / per;
-      it.chunk_no = by_tile ? 0 : in - it.tile * per;
-      it.chunk = chunk;
-      it.q0 = pick(l.q0);
-      it.rows = pick(l.rows);
-      it.len = pick(l.len);
-      it.over = pick((int)l.over);
-      it.slot = pick(slot_end - n_slots) + it.tile * per;
-      // the last tiles of a prompt see the most: they go first
-      it.tile = pick(l.tiles) - 1 - it.tile;
-      return true;
+    if (!hit) return false;
+    it.b = __ffsll(hit) - 1;
+    auto pick = [&](int v) { return __builtin_amdgcn_readlane(v, it.b); };
+    in = want - pick(end - count);
+    slot = pick(slot_end - c.slots);
+    l = Load{pick(mine.q0), pick(mine.rows), pick(mine.len), pick(mine.tiles), pick(mine.units), pick((int)mine.over) != 0};
+  } else {
+    // the first request whose running count is over `want`: 64 of them at a time, then those up to it
+    const int4* ends = (const int4*)((const char*)a.plan + kEnds);
+    auto end_of = [&](int b) { return by_tile ? ends[b].y : ends[b].x; };
+    const int step = (a.B + kWave - 1) / kWave;
+    unsigned long long over = __ballot(end_of(min((lane + 1) * step, a.B) - 1) > want);
+    if (!over) return false;
+    const int lo = (__ffsll(over) - 1) * step, hi = min(lo + step, a.B);
+    for (int b0 = lo;; b0 += kWave) {
+      over = __ballot(end_of(min(b0 + lane, hi - 1)) > want);
+      it.b = min(b0 + (over ? __ffsll(over) - 1 : 0), hi - 1);
+      if (over || b0 + kWave >= hi) break;
     }
-    (by_tile ? tiles : items) = __builtin_amdgcn_readlane(end, kWave - 1);
-    slots = __builtin_amdgcn_readlane(slot_end, kWave - 1);
+    const int4 before = it.b > 0 ? ends[it.b - 1] : make_int4(0, 0, 0, 0);
+    in = want - (by_tile ? before.y : before.x);
+    slot = before.z;
+    l = load_of<RT>(a, it.b);
   }
-  return false;
+  const int per = max(ceil_div(l.units, chunk), 1);
+  const int tile = by_tile ? in : in / per;
+  it.chunk_no = by_tile ? 0 : in - tile * per;
+  it.chunk = chunk;
+  it.q0 = l.q0;
+  it.rows = l.rows;
+  it.len = l.len;
+  it.over = l.over;
+  it.slot = slot + tile * per;
+  it.tile = l.tiles - 1 - tile;  // the last tiles of a prompt see the most: they go first
+  for (int* f : {&it.b, &it.tile, &it.chunk_no, &it.q0, &it.rows, &it.len, &it.slot})
+    *f = __builtin_amdgcn_readfirstlane(*f);
+  return true;
 }
 
 // What a tile's columns see: units [lo, hi), and how many chunks they are cut into.
@@ -337,18 +402,28 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
 
   const int wave = uniform(threadIdx.x >> 6);
   const int hk = blockIdx.x % a.Hk;
-  const int chunk = chunk_of<RT>(a);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.chunk = chunk;
+  const int chunk = a.B <= kWave ? chunk_of_few<RT>(a) : *a.plan;
+  if (a.B <= kWave && blockIdx.x == 0 && threadIdx.x == 0) *a.plan = chunk;  // for the join
   Item it;
   for (int want = blockIdx.x / a.Hk; find_item<RT>(a, chunk, want, false, it); want += gridDim.x / a.Hk) {
   const Span sp = span_of<RT>(a, it);
+  const int r0 = it.tile * RT, n_cols = min(RT, it.rows * a.G - r0);
+  if (it.over) {
+    if (it.chunk_no == 0) {
+      const uint32_t nan = F16 ? 0x7e007e00u : 0x7fc07fc0u;
+      for (int e = threadIdx.x; e < n_cols * (D / 8); e += kThreads) {
+        const int c = e / (D / 8), r = r0 + c, row = r / a.G, head = hk * a.G + (r - row * a.G);
+        *(uint4*)((uint16_t*)a.out + (it.q0 + row) * a.o_st + head * a.o_sh + (e - c * (D / 8)) * 8) =
+            make_uint4(nan, nan, nan, nan);
+      }
+    }
+    continue;
+  }
   if (it.chunk_no >= sp.chunks || (sp.chunks > 1 && it.slot + sp.chunks > a.max_slots)) continue;
   __syncthreads();  // the item before is done with LDS
   const int lane = this_lane();
   const int i16 = lane & 15, g = lane >> 4;
   const int page_mask = (1 << a.log_page) - 1;
-  const int r0 = it.tile * RT;
-  const int n_cols = min(RT, it.rows * a.G - r0);
 
   // ---- Q as operand B: column i, dimensions 64 s + 16 g + 8 h ... of step 2 s + h
   frag qf[kQLds ? 1 : CT][kQLds ? 1 : 2 * KS];
@@ -397,7 +472,7 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
     r.v = a.vc + (((vq * a.Hk + hk) * D + i16) << a.log_page) + ((tok + 16 * g) & page_mask);
     r.ks = a.ks[vq * a.Hk + hk];
     r.vs = a.vs[vq * a.Hk + hk];
-    if (bad || it.over) r.ks = r.vs = __uint_as_float(0x7fc00000u);
+    if (bad) r.ks = r.vs = __uint_as_float(0x7fc00000u);
     return r;
   };
   const int u_end = uniform(min(sp.lo + (it.chunk_no + 1) * it.chunk, sp.hi));
@@ -639,11 +714,11 @@ __global__ __launch_bounds__(kThreads) void kv_attention_join_kernel(AttnArgs a)
   __shared__ f32x4_t part_o[kWaves][kWave];
   __shared__ float part_m[kWaves][kWave], part_l[kWaves][kWave];
   const int hk = blockIdx.x % a.Hk;
-  const int chunk = *a.chunk;
+  const int chunk = *a.plan;
   Item it;
   if (!find_item<RT>(a, chunk, blockIdx.x / a.Hk, true, it)) return;
   const Span sp = span_of<RT>(a, it);
-  if (sp.chunks == 1 || it.slot + sp.chunks > a.max_slots) return;
+  if (it.over || sp.chunks == 1 || it.slot + sp.chunks > a.max_slots) return;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int n_cols = min(RT, it.rows * a.G - it.tile * RT);
   const float* ml = a.part + (size_t)a.max_slots * a.Hk * RT * D;
@@ -730,16 +805,19 @@ Grid grid_of(int T, int B, int Hq, int Hk, int D, int64_t tokens) {
   return r;
 }
 
-constexpr size_t kHeader = 64;  // bytes of the workspace in front of the partial sums
+// Bytes of the workspace in front of the partial sums.
+size_t plan_bytes(int B) { return kEnds + (B > kWave ? ((size_t)B * sizeof(int4) + 63) / 64 * 64 : 0); }
 
-size_t part_bytes(const Grid& gr, int Hk, int D) {
-  return kHeader + (size_t)gr.max_slots * Hk * gr.ct * 16 * (D + 2) * sizeof(float);
+size_t part_bytes(const Grid& gr, int B, int Hk, int D) {
+  return plan_bytes(B) + (size_t)gr.max_slots * Hk * gr.ct * 16 * (D + 2) * sizeof(float);
 }
 
 bool width_ok(int D) { return D == 64 || D == 128 || D == 256 || D == 512; }
 
 template <int D, int CT, bool F16>
 void launch(const AttnArgs& a, const Grid& gr, hipStream_t stream) {
+  if (a.B > kWave)
+    hipLaunchKernelGGL(kv_attention_plan_kernel<16 * CT>, dim3(1), dim3(kPlanThreads), 0, stream, a);
   hipLaunchKernelGGL((kv_attention_kernel<D, CT, F16>), dim3(gr.groups * a.Hk), dim3(kThreads), 0, stream, a);
   // up to 2048 workgroups, each for as many of its tile's values as that leaves
   if (gr.max_slots == 0) return;
@@ -767,7 +845,7 @@ void launch_d(const AttnArgs& a, const Grid& gr, int D, hipStream_t stream) {
 
 size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D, int64_t max_tokens) {
   if (T <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || !width_ok(D) || max_tokens < 0) return 0;
-  return part_bytes(grid_of(T, B, Hq, Hk, D, max_tokens), Hk, D);
+  return part_bytes(grid_of(T, B, Hq, Hk, D, max_tokens), B, Hk, D);
 }
 
 int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, const void* k_cache, const void* v_cache,
@@ -798,13 +876,15 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
     if ((uintptr_t)p & 15) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
   for (const int64_t s : {q_strides[0], q_strides[1], o_strides[0], o_strides[1]})
     if (s % 8) return fail(GI_ERR_INVALID_ARG, "kv_attention: row and head strides must be multiples of 8 elements");
+  if (window >= (int64_t)max_pages * page_size) window = 0;  // no request is that long
+  if ((uintptr_t)workspace & 15) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
   const Grid gr = grid_of(T, B, Hq, Hk, D, (int64_t)max_pages * page_size);
   if ((int64_t)gr.groups * Hk > 0x7fffffff) return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows");
-  if (!workspace || workspace_bytes < part_bytes(gr, Hk, D))
+  if (!workspace || workspace_bytes < part_bytes(gr, B, Hk, D))
     return fail(GI_ERR_WORKSPACE, "kv_attention: workspace missing or too small");
   AttnArgs a{q, q_strides[0], q_strides[1], (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale,
              block_table, table_stride, seq_lens, q_start, out, o_strides[0], o_strides[1], (int*)workspace,
-             (float*)((char*)workspace + kHeader),
+             (float*)((char*)workspace + plan_bytes(B)),
              num_pages, scale * kLog2e, T, B, Hk, Hq / Hk, max_pages, lp, window, gr.resident, gr.max_slots};
   if (dtype == GI_DTYPE_FP16) launch_d<true>(a, gr, D, stream);
   else launch_d<false>(a, gr, D, stream);

@@ -382,13 +382,21 @@ def test_attention_row_tiles(rows, hq, hk, d):
     _check_attention([rows + 111, rows], [rows, rows], hq, hk, 32, d, BF16, seed=rows)
 
 
-@pytest.mark.parametrize("b", [65, 130, 300])
+@pytest.mark.parametrize("b", [64, 65, 130, 300, 4100])
 def test_attention_many_requests(b):
     rng = random.Random(b)
     lens = [rng.choice([0, 1, 5, 60, 100]) for _ in range(b)]
     _check_attention(lens, [1] * b, 2, 1, 16, 64, BF16, seed=b, decode=True)
     rows = [rng.choice([0, 1, 2]) for _ in range(b)]
     _check_attention([n + r for n, r in zip(lens, rows)], rows, 2, 1, 16, 64, BF16, seed=b)
+
+
+def test_attention_long_request_among_many():
+    """A request over many workgroups beside 99 short ones: its partial sums are where the join looks."""
+    lens = [30] * 100
+    lens[37] = 20000
+    _check_attention(lens, [1] * 100, 8, 2, 64, 64, BF16, seed=8, decode=True, spread=2.0)
+    _check_attention(lens, [3] * 100, 8, 2, 64, 64, FP16, seed=9)
 
 
 @pytest.mark.parametrize("hq,hk,d,rows", [(16, 8, 256, 1), (16, 2, 512, 1), (4, 2, 64, 3), (8, 1, 128, 40)])
@@ -468,6 +476,23 @@ def test_attention_missing_pages_and_poisoned_scales_give_nan():
     assert torch.isnan(got[:180]).all() and torch.equal(got[180:], clean[180:])
     got = ops.kv_attention(q, dev, _i32(table), _i32([2 ** 31 - 1] * 4), _i32(start))
     assert torch.isnan(got).all()
+    # more rows than the table has room for, and a table without room
+    for cols in (1, 0):
+        got = ops.kv_attention(q, dev, _i32(table)[:, :cols], _i32(lens), _i32(start), window=7)
+        assert torch.isnan(got).all()
+    got = ops.kv_attention(q, dev, _i32(table)[:, :0], _i32([0, -3, 0, 0]), _i32(start))
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 64, 63])
+def test_attention_windows_around_the_table(window):
+    """Windows as long as the table and longer, with rows that see nothing beside ones that do."""
+    lens, rows, page = [40, 20, 48], [60, 3, 48], 16
+    cache, table, start = _setup(lens, rows, 1, page, 64, seed=5)
+    q = torch.randn(start[-1], 2, 64, generator=_gen(4)).to(BF16)
+    got = ops.kv_attention(q.to(DEV), _to(cache, DEV), _i32(table), _i32(lens), _i32(start), window=window)
+    ref, weighted, size = O.attention(q, cache, table, lens, start, 64 ** -0.5, window)
+    _check_out(got, ref, weighted, size, 64, 48)
 
 
 def test_attention_leaves_rows_behind_the_last_request():
