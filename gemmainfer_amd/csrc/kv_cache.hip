@@ -32,7 +32,7 @@ namespace {
 // ---------------------------------------------------------------------------
 // One launch, no exchange between workgroups: each scans the B request lengths
 // into its own LDS (12 bytes of global reads a request) and then places its
-// 256 tokens.  A fresh page j of a request starts at position j*P >= ctx, which
+// 256 tokens (7 requests 3.4 us, 301 requests and 14,500 rows 5.5 us).  A fresh page j of a request starts at position j*P >= ctx, which
 // is one of the call's own tokens: that token's thread writes the table entry,
 // so table entries are never read and written in one call.  Bound by latency
 // (lengths -> scan -> table entry -> slot).
@@ -245,8 +245,9 @@ __device__ __forceinline__ float page_scale(uint32_t amax_bits) {
 // a slot is named twice), the largest value of those rows, the page's scale,
 // then the codes.  Everything of a page in one workgroup needs no atomics on
 // scales and no second launch.  A decode step is bound by latency (slots, then
-// rows and scale, then stores), a prompt by HBM; the rows are read twice, the
-// second time from the caches.  per_wg rows are looked at by one workgroup.
+// rows and scale, then stores: 61 rows of 8 heads of 256 in 6 us), a prompt by its rows' two
+// reads (6000 rows: 27 us, 74 MB in and out; kept in registers instead, fewer workgroups fit and it
+// takes 34).  per_wg rows are looked at by one workgroup.
 template <typename T, bool kVec>
 __global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
   __shared__ int last[kMaxPage];               // the row on each place, -1: none
