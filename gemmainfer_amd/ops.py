@@ -662,8 +662,9 @@ def kv_slots(ctx_lens, new_lens, block_table, free_pages, free_used, page_size, 
     """Places the new tokens of B requests on cache pages, on the device.
 
     ``ctx_lens``/``new_lens`` int32 [B]: tokens in the cache, tokens to add.
-    ``block_table`` int32 [B, max_pages] is written where the step opens pages,
-    which come from ``free_pages`` (int32) behind the first ``free_used[0]`` of
+    ``block_table`` int32 [B, max_pages] is written where the step opens pages
+    (those from token ceil(ctx / page) * page on, whatever stood there), which
+    come from ``free_pages`` (int32) behind the first ``free_used[0]`` of
     them.  ``num_rows`` rows are laid out (the packed rows of q, k and v,
     request after request); those behind the last request get slot -1 and
     position 0.  A row without a page gets slot -1; ``status`` counts what was
@@ -682,7 +683,8 @@ def kv_slots(ctx_lens, new_lens, block_table, free_pages, free_used, page_size, 
         raise ValueError(f"kv_slots: num_rows must be in [0, 2^31), got {num_rows}")
     cols, stride = _table(block_table, b, "kv_slots")
     slots, positions = torch.empty((2, num_rows), dtype=torch.int64, device=dev).unbind(0)
-    q_start, seq_lens, status = torch.empty(2 * b + 4, dtype=torch.int32, device=dev).split((b + 1, b, 3))
+    q_start, seq_lens, status = torch.split_with_sizes(torch.empty(2 * b + 4, dtype=torch.int32, device=dev),
+                                                       (b + 1, b, 3))
     _launch(dev, "kv_slots",
         ctx_lens.data_ptr(), new_lens.data_ptr(), b, block_table.data_ptr(), cols, stride, free_pages.data_ptr(),
         free_pages.numel(), free_used.data_ptr(), page_size, slots.data_ptr(), positions.data_ptr(), num_rows,

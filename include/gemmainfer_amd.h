@@ -377,7 +377,9 @@ int gi_rope_rows(const void* q, void* q_out, const void* k, void* k_out,
  *                        request get slot -1 and position 0
  *   block_table          entries of the pages that the step opens are written
  * Pages are taken from free_pages[free_used[0] ...] in the order of the
- * requests; none is taken for a page that holds tokens already.  status int32
+ * requests; none is taken for a page that holds tokens already (a page behind
+ * the ctx_lens[b] tokens is opened anew, whatever its table entry was: after a
+ * rollback over a page's end the caller puts that page back).  status int32
  * [3] = {free_used after the step, pages that were lacking (the list was used
  * up, or the request needs more than max_pages), rows past n_tokens that were
  * dropped}.  A row whose page is lacking gets slot -1, and its table entry -1.
