@@ -39,6 +39,9 @@ constexpr int kEnds = 64;      // bytes of the plan in front of the running coun
 // what a compute unit holds of a kernel: by its registers, two waves a SIMD or one
 constexpr int workgroups_per_cu(int D, int CT) { return D * CT <= (CT == 1 ? 256 : 128) ? 2 : 1; }
 constexpr float kLog2e = 1.4426950408889634f;
+// The partial sums fit the workspace while choose_chunk's total is right to 1e-4: over this
+// many requests, 1024 to a thread, an fp32 sum is off by at most about 2^10 * 2^-24.
+constexpr int kMaxRequests = 1 << 20;
 // Weights go to the matrix cores in fp16 as 2^(t - m + kBias).  The reference m
 // is a maximum of earlier rows and follows when a lane's 16 weights sum to more than
 // kMostSum, so none is over 2^15; fp16 is normal down to 2^-14, so a weight
@@ -871,6 +874,7 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
     if (page_size == 1 << l) lp = l;
   if (lp < 0) return fail(GI_ERR_INVALID_ARG, "kv_attention: page_size must be 16, 32, 64, 128 or 256");
   if (!q_start && T != B) return fail(GI_ERR_INVALID_ARG, "kv_attention: without q_start there is one row a request");
+  if (B > kMaxRequests) return fail(GI_ERR_UNSUPPORTED, "kv_attention: at most 2^20 requests");
   if (!(scale == scale)) return fail(GI_ERR_INVALID_ARG, "kv_attention: scale is NaN");
   if (window < 0) return fail(GI_ERR_INVALID_ARG, "kv_attention: window must be >= 0 (0: none)");
   if ((int64_t)T * (Hq / Hk) > 0x3fffffff || (int64_t)max_pages * page_size > 0x3fffffff)

@@ -436,6 +436,7 @@ int launch_kv_append(const void* k, const void* v, int dtype, const int64_t* k_s
   if (T < 0 || Hk <= 0 || num_pages < 0 || D <= 0 || D % 8 || D > 1024)
     return fail(GI_ERR_INVALID_ARG, "kv_append: T, num_pages >= 0, Hk > 0 and D a multiple of 8 up to 1024 required");
   if (Hk > 65535) return fail(GI_ERR_UNSUPPORTED, "kv_append: at most 65535 kv heads");
+  if (T > 1 << 30) return fail(GI_ERR_UNSUPPORTED, "kv_append: at most 2^30 rows");
   if (T == 0 || num_pages == 0) return GI_OK;
   if (!k || !v || !slots || !k_cache || !v_cache || !k_scale || !v_scale)
     return fail(GI_ERR_INVALID_ARG, "kv_append: null pointer");

@@ -112,6 +112,16 @@ def test_kv_attention_refuses(lib, over, code, frag):
     assert st == code and (code == L.GI_OK or frag in msg)
 
 
+def test_largest_counts_are_refused(lib):
+    """Where the kernels' own counting would end: refused before any pointer is looked at."""
+    st, msg = _call(lib, "gi_kv_append", APPEND, dict(T=(1 << 30) + 1, k=None))
+    assert st == L.GI_ERR_UNSUPPORTED and "2^30" in msg
+    st, msg = _call(lib, "gi_kv_attention", ATTN, dict(B=(1 << 20) + 1, q=None))
+    assert st == L.GI_ERR_UNSUPPORTED and "2^20" in msg
+    st, msg = _call(lib, "gi_kv_attention", ATTN, dict(B=1 << 20, T=1 << 20, start=None))
+    assert st == L.GI_ERR_WORKSPACE
+
+
 def test_workspace_query_is_host_only(lib):
     q = lib.gi_kv_attention_workspace_bytes
     for bad in ((0, 1, 16, 8, 256), (1, 0, 16, 8, 256), (1, 1, 15, 8, 256), (1, 1, 16, 8, 96)):
