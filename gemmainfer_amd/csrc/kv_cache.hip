@@ -18,6 +18,7 @@
 // where they fall under e4m3's smallest normal number).
 
 #include <numeric>
+#include <type_traits>
 
 #include "../../include/gemmainfer_amd.h"
 #include "gi_common.h"
@@ -160,6 +161,9 @@ __global__ __launch_bounds__(kSlotThreads) void kv_slots_kernel(SlotArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int kAppThreads = 256;
 constexpr int kMaxPage = 256;
+// slots a lane loads at a time where it looks for a run's start or end over skipped rows (with eight the
+// kernel takes 92 registers instead of 76: 1024 decoded rows 47 us, with four 42)
+constexpr int kLookRows = 4;
 
 struct AppendArgs {
   const void* x[2];        // K rows, V rows
@@ -240,8 +244,8 @@ __device__ __forceinline__ float page_scale(uint32_t amax_bits) {
 }
 
 // One workgroup a (run of rows, head, K or V); a run is the rows of the call
-// that follow each other on one page, and its first row's workgroup does it
-// all: which row lands on each of the page's P places (the last one wins where
+// that follow each other on one page, rows that are skipped between them or not,
+// and its first row's workgroup does it all: which row lands on each of the page's P places (the last one wins where
 // a slot is named twice), the largest value of those rows, the page's scale,
 // then the codes.  Everything of a page in one workgroup needs no atomics on
 // scales and no second launch.  A decode step is bound by latency (slots, then
@@ -260,33 +264,71 @@ __global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
   const T* x = (const T*)a.x[kv] + head * a.sh[kv];
   const int64_t st = a.st[kv];
   const int t_first = (int)(blockIdx.x * a.spread % gridDim.x) * a.per_wg;
-  // the first rows of runs among this workgroup's rows (every wave finds them all)
+  auto on_page = [&](int64_t s) { return s >= 0 && s >> lp < a.num_pages; };
+  // the first rows of runs among this workgroup's rows (every wave finds them
+  // all): those whose page is not that of the last row before them that has one.
+  // Lanes 0 ... back - 1 look at the rows in front of the workgroup's own.
+  const int back = kWave - a.per_wg, t_look = t_first - back;
   unsigned long long runs;
   {
-    const int t = t_first + lane;
-    const int64_t s = lane < a.per_wg && t < a.T ? a.slots[t] : -1;
-    const int64_t before = t > 0 && t < a.T ? a.slots[t - 1] : -1;
-    runs = __ballot(s >= 0 && s >> lp < a.num_pages && (before < 0 || before >> lp != s >> lp));
+    const int t = t_look + lane;
+    const int64_t s = t >= 0 && t < a.T ? a.slots[t] : -1;
+    const bool ok = on_page(s);
+    const unsigned long long oks = __ballot(ok), below = oks & ((1ull << lane) - 1);
+    const long long page = s >> lp, before = __shfl(page, below ? 63 - __clzll(below) : lane, kWave);
+    runs = __ballot(ok && lane >= back && (!below || before != page));
+    const int first = oks ? __ffsll(oks) - 1 : 0;
+    if (first >= back && runs) {
+      // nothing but skipped rows in sight of it: further back, 256 rows at a time
+      const long long its = __shfl(page, first, kWave);
+      bool found = false;
+      for (int end = t_look; end > 0 && !found; end -= kLookRows * kWave) {
+        int64_t p[kLookRows];
+#pragma unroll
+        for (int i = 0; i < kLookRows; ++i) p[i] = end - 1 - i * kWave - lane >= 0 ? a.slots[end - 1 - i * kWave - lane] : -1;
+#pragma unroll
+        for (int i = 0; i < kLookRows; ++i) {
+          const unsigned long long hit = __ballot(on_page(p[i]));
+          if (found || !hit) continue;
+          found = true;
+          if (__shfl((long long)(p[i] >> lp), __ffsll(hit) - 1, kWave) == its) runs &= ~(1ull << first);
+        }
+      }
+    }
   }
   for (; runs; runs &= runs - 1) {
-    const int t0 = t_first + __ffsll(runs) - 1;
+    const int t0 = t_look + __ffsll(runs) - 1;
     const int64_t page = a.slots[t0] >> lp;
     float* scale = a.scale[kv] + page * a.Hk + head;
     const float old = *scale;
     __syncthreads();  // the run before is done with LDS
     if (tid < P) last[tid] = -1;
-    // ---- the run's rows
-    for (int base = t0;; base += kAppThreads) {
-      const int t = base + tid;
-      const int64_t s = t < a.T ? a.slots[t] : -1;
-      const unsigned long long other = __ballot(s < 0 || s >> lp != page);
-      if (lane == 0) wave_end[wave] = other ? base + wave * kWave + __ffsll(other) - 1 : 0x7fffffff;
+    // ---- the run's rows: those on the page up to the first one of another page
+    auto look = [&](int base, auto count) {  // at `count` rows a thread; true where the run ends
+      constexpr int kRows = decltype(count)::value;
+      int64_t s[kRows];
+      int end = 0x7fffffff;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) s[i] = base + i * kAppThreads + tid < a.T ? a.slots[base + i * kAppThreads + tid] : -1;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const unsigned long long other = __ballot(on_page(s[i]) && s[i] >> lp != page);
+        if (other) end = min(end, base + i * kAppThreads + wave * kWave + __ffsll(other) - 1);
+      }
+      if (lane == 0) wave_end[wave] = end;
       __syncthreads();
-      const int end = min(min(wave_end[0], wave_end[1]), min(wave_end[2], wave_end[3]));
-      if (t < end) atomicMax(&last[s & (P - 1)], t);
+      end = min(min(wave_end[0], wave_end[1]), min(wave_end[2], wave_end[3]));
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int t = base + i * kAppThreads + tid;
+        if (t < end && s[i] >= 0 && s[i] >> lp == page) atomicMax(&last[s[i] & (P - 1)], t);
+      }
       __syncthreads();
-      if (end != 0x7fffffff) break;
-    }
+      return end != 0x7fffffff || base + kRows * kAppThreads >= a.T;
+    };
+    if (!look(t0, std::integral_constant<int, 1>()))
+      for (int base = t0 + kAppThreads; !look(base, std::integral_constant<int, kLookRows>()); base += kLookRows * kAppThreads) {
+      }
     const bool on = tid < P && last[tid] >= 0;
     const unsigned long long bits = __ballot(on);
     if (lane < 4 && wave * 4 + lane < P >> 4) group_rows[wave * 4 + lane] = (uint32_t)(bits >> (16 * lane)) & 0xffffu;

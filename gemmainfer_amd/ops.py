@@ -775,8 +775,9 @@ def kv_append(k, v, slots, cache: KVCache) -> None:
     """Stores rows k and v [T, Hk, D] (bf16/fp16/fp32) in the cache at ``slots``
     (int64 [T]; negative ones, and those past the last page, are skipped).
 
-    The rows of one page must follow each other, as those of a request do; of
-    rows with the same slot the last one is stored.  Each page has one scale per
+    The rows of one page must follow each other, as those of a request do
+    (skipped rows may stand between them); of rows with the same slot the last
+    one is stored.  Each page has one scale per
     head for K and one for V, a power of two that grows as larger rows arrive
     (what the page holds is then rounded to the new one); writing a page's first
     place starts the page anew.  A row with an infinity or NaN makes its page's

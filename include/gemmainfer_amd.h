@@ -394,8 +394,9 @@ int gi_kv_slots(const int32_t* ctx_lens, const int32_t* new_lens, int B,
 /* Writes rows of K and V ([T, Hk, D], last dimension contiguous, strides in
  * elements; bf16, fp16 or fp32) into their slots.  Slots that are negative or
  * past the last page are skipped.  The rows of one page must follow each other
- * in the call (those of a request do); of rows with the same slot the last one
- * is stored.  A page's scale (per head, K and V apart) is the smallest power of two, at
+ * in the call (those of a request do), with no row of another page between them;
+ * skipped rows may stand there.  Of rows with the same slot the last one is
+ * stored.  A page's scale (per head, K and V apart) is the smallest power of two, at
  * least 2^-40, that brings its largest value to at most 448.  Writing a page's
  * first place starts the page anew, with the scale of the rows of this call;
  * otherwise the scale only grows, and what the page holds is rounded to the

@@ -254,6 +254,68 @@ def test_append_skips_duplicates_and_bad_slots():
     _check_append(cache, e, e, [])
 
 
+def _sized_rows(t, hk, d, seed):
+    """Rows whose sizes differ by powers of two, so that rows all along a run raise its page's scale."""
+    g = _gen(seed)
+    size = torch.exp2(3 * torch.randn(t, hk, 1, generator=g))
+    return ((torch.randn(t, hk, d, generator=g) * size).to(BF16) for _ in range(2))
+
+
+@pytest.mark.parametrize("hk", [2, 700])
+def test_append_skipped_rows_inside_a_page(hk):
+    """Rows of one page with skipped ones between them are one run: the page's scale is that of them
+    all, whichever raises it.  2 heads: a workgroup a row; 700: sixteen rows a workgroup."""
+    page, pages = 16, 5
+    cache = _filled(pages, hk, page, 8, seed=hk)
+    for slots in ([17, -1, 18], [-1, 17, -1, -9, 18, -1], [17, pages * page, 1 << 40, 18, -(1 << 40), 19],
+                  [20, -1, 33, -1, 34, -1, 48, -1, 49, -1], [-1, -1, 18, 19, -1, 20, -1, -1, 21, 36, -1, 37, -1, 38, 70, -1]):
+        slots = slots + [-1] * (16 - len(slots))
+        n = len(slots)
+        rows = torch.exp2(torch.arange(n).float() * 2 - 6).view(n, 1, 1) * torch.ones(n, hk, 8)
+        _check_append(cache, rows.to(BF16), rows.flip(0).to(BF16), slots)
+        k, v = _sized_rows(n, hk, 8, n)
+        _check_append(cache, k, v, slots)
+
+
+@pytest.mark.parametrize("hk", [1, 40])
+@pytest.mark.parametrize("hole", [14, 15, 16, 47, 48, 62, 63, 64, 65, 255, 256, 257, 511, 512, 513, 575, 576, 2303, 2304,
+                                  2305, 5000])
+def test_append_holes_of_any_length(hk, hole):
+    """Skipped rows before, between and behind the rows of a page, over every number of rows that is
+    looked at together."""
+    page = 16
+    cache = _filled(6, hk, page, 8, seed=hole)
+    for slots in ([17] + [-1] * hole + [18, 19, 35],                              # one page on both sides
+                  [17] + [-1] * hole + [33, 34] + [6 * page] * hole + [35],      # another behind it, then one again
+                  [-1] * hole + [49] + [-1] * hole):
+        k, v = _sized_rows(len(slots), hk, 8, hole)
+        _check_append(cache, k, v, slots)
+
+
+@pytest.mark.parametrize("page,hk,t", [(16, 2, 900), (16, 40, 900), (64, 40, 2000), (256, 33, 1500)])
+def test_append_random_runs_and_holes(page, hk, t):
+    """Pages in any order, runs of 1 to 40 rows in any order of places (some named twice), holes of
+    1 to 90 rows anywhere."""
+    rng = random.Random(page * hk)
+    pages = 700
+    ids = list(range(pages))
+    rng.shuffle(ids)
+    slots = []
+    while len(slots) < t:
+        p = ids.pop()
+        for _ in range(rng.choice([1, 1, 1, 2, 7, 16, 40])):
+            slots.append(p * page + rng.randrange(page))
+            if rng.random() < 0.1:
+                slots += [-1] * rng.choice([1, 1, 2, 15, 90])
+        slots += [-1] * rng.choice([0, 0, 0, 1, 5, 70])
+    cache = _filled(pages, 2, page, 8, seed=page)
+    cache = ops.KVCache(*[x.repeat_interleave(-(-hk // 2), 1)[:, :hk].contiguous() if x.dtype == FP32 else
+                          x.view(torch.uint8).repeat_interleave(-(-hk // 2), 1)[:, :hk].contiguous().view(O.E4M3)
+                          for x in cache])
+    k, v = _sized_rows(len(slots), hk, 8, t)
+    _check_append(cache, k, v, slots)
+
+
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan"), 3e38, 448.0 * 2 ** 40, 2.0 ** -133, 0.0])
 def test_append_extreme_values(value):
     page, d = 16, 64
