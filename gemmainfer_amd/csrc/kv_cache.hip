@@ -164,6 +164,7 @@ constexpr int kMaxPage = 256;
 // slots a lane loads at a time where it looks for a run's start or end over skipped rows (with eight the
 // kernel takes 92 registers instead of 76: 1024 decoded rows 47 us, with four 42)
 constexpr int kLookRows = 4;
+constexpr uint32_t kAppGrid = 1u << 23;  // workgroups along x: with their threads under the 2^32 that a launch may have
 
 struct AppendArgs {
   const void* x[2];        // K rows, V rows
@@ -173,7 +174,7 @@ struct AppendArgs {
   float* scale[2];
   int64_t num_pages;
   int T, Hk, D, log_page, per_wg;
-  uint32_t spread;         // workgroup i looks at rows (i * spread mod their number) * per_wg ...
+  uint32_t blocks, spread;  // workgroup i of `blocks` looks at rows (i * spread mod blocks) * per_wg ...
 };
 
 template <typename T>
@@ -259,11 +260,13 @@ __global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
   __shared__ uint32_t group_rows[kMaxPage / 16];  // ... as bits of each 16 places
   __shared__ uint32_t wave_max[kAppThreads / kWave];
   __shared__ int wave_end[kAppThreads / kWave], wave_count[kAppThreads / kWave];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y, kv = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, head = blockIdx.y, kv = blockIdx.z & 1;
+  const uint32_t block = (blockIdx.z >> 1) * gridDim.x + blockIdx.x;
+  if (block >= a.blocks) return;
   const int lp = a.log_page, P = 1 << lp, D = a.D;
   const T* x = (const T*)a.x[kv] + head * a.sh[kv];
   const int64_t st = a.st[kv];
-  const int t_first = (int)(blockIdx.x * a.spread % gridDim.x) * a.per_wg;
+  const int t_first = (int)(block * a.spread % a.blocks) * a.per_wg;
   auto on_page = [&](int64_t s) { return s >= 0 && s >> lp < a.num_pages; };
   // the first rows of runs among this workgroup's rows (every wave finds them
   // all): those whose page is not that of the last row before them that has one.
@@ -508,6 +511,7 @@ int launch_kv_append(const void* k, const void* v, int dtype, const int64_t* k_s
   // would all fall on a few of the chip's eight parts (6000 rows onto pages of
   // 64: 29.8 us, spread out 27.7).
   const uint32_t blocks = (uint32_t)((T - 1) / a.per_wg + 1);
+  a.blocks = blocks;
   a.spread = 1;
   if (a.per_wg > 1 && blocks < 1u << 25) {
     a.spread = 61;
@@ -516,7 +520,8 @@ int launch_kv_append(const void* k, const void* v, int dtype, const int64_t* k_s
   const int size = dtype == GI_DTYPE_FP32 ? 4 : 2;
   bool vec = aligned16(k) && aligned16(v);
   for (int i = 0; i < 2; ++i) vec = vec && a.st[i] * size % 16 == 0 && a.sh[i] * size % 16 == 0;
-  const dim3 grid(blocks, Hk, 2);
+  const uint32_t width = blocks < kAppGrid ? blocks : kAppGrid;
+  const dim3 grid(width, Hk, 2 * ((blocks - 1) / width + 1));
 #define GI_APPEND(T_)                                                                                        \
   do {                                                                                                       \
     if (vec) hipLaunchKernelGGL((kv_append_kernel<T_, true>), grid, dim3(kAppThreads), 0, stream, a);        \

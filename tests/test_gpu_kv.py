@@ -352,6 +352,25 @@ def test_append_rounds_and_rescales_every_code():
     _check_append(cache, x, x, list(range(2 * page, 2 * page + x.shape[0])))
 
 
+def test_append_more_rows_than_a_grid_is_wide():
+    """2^28 rows and more, 2^20 to a page: of each place the last one stays."""
+    t, group, page, d = (1 << 28) + (1 << 20) + 5, 1 << 20, 16, 8
+    row = torch.arange(t, device=DEV)
+    slots = row // group * page + row % page
+    x = torch.empty(t, 1, d, dtype=BF16, device=DEV)
+    x[:] = (row % 1009).to(BF16)[:, None, None]
+    pages = t // group + 1
+    cache, want = ops.kv_cache(pages, 1, page, d * 8, DEV), ops.kv_cache(pages, 1, page, d * 8, DEV)
+    cache, want = (c._replace(k=c.k[..., :d].contiguous(), v=c.v[:, :, :d].contiguous()) for c in (cache, want))
+    ops.kv_append(x, -x, slots, cache)
+    ends = [min((p + 1) * group, t) for p in range(pages)]
+    last = torch.cat([torch.arange(max(e - page, p * group), e) for p, e in enumerate(ends)]).to(DEV)
+    assert pages == 258 and last.numel() == 257 * page + 5
+    ops.kv_append(x[last], -x[last], slots[last], want)
+    for a, b in zip(cache, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_append_strided_rows():
     page, d, hk, t = 16, 128, 2, 21
     cache = _filled(5, hk, page, d, seed=8)
