@@ -101,6 +101,7 @@ __global__ __launch_bounds__(256) void rope_kernel(T* q, T* k, const T* cs, cons
 // element is read and written once.
 constexpr int kRopeThreads = 256;
 constexpr int kRopeMaxPairs = 512;
+constexpr int kRopeGrid = 1 << 23;  // rows along x: with a row's threads under the 2^32 that a launch may have
 
 struct RopeArgs {
   const void* in[2];   // q, k
@@ -109,7 +110,7 @@ struct RopeArgs {
   const int64_t* pos;
   const double* freq;
   float mscale;
-  int heads[2], D, pairs;
+  int T, heads[2], D, pairs;
   int turn, units;     // units of a head that turn, and with those that are only copied
 };
 
@@ -134,7 +135,8 @@ template <typename T, bool kInter, bool kVec>
 __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeArgs a) {
   constexpr int N = kVec ? 8 : 1;
   __shared__ float cs[kRopeMaxPairs], sn[kRopeMaxPairs];
-  const int64_t row = blockIdx.x;
+  const int64_t row = (int64_t)blockIdx.z * gridDim.x + blockIdx.x;
+  if (row >= a.T) return;
   const int R = 2 * a.pairs;
   const int i = blockIdx.y * kRopeThreads + threadIdx.x;
   const int h = i / a.units, u = i - h * a.units;
@@ -273,7 +275,7 @@ int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, con
   if ((Hq > 0 && (!q || !q_out)) || (Hk > 0 && !k_out) || !positions || !inv_freq)
     return fail(GI_ERR_INVALID_ARG, "rope_rows: null pointer");
   RopeArgs a{{q, k}, {q_out, k_out}, {q_strides[0], k_strides[0]}, {q_strides[1], k_strides[1]},
-             {qo_strides[0], ko_strides[0]}, {qo_strides[1], ko_strides[1]}, positions, inv_freq, mscale, {Hq, Hk}, D,
+             {qo_strides[0], ko_strides[0]}, {qo_strides[1], ko_strides[1]}, positions, inv_freq, mscale, T, {Hq, Hk}, D,
              rotary_dim / 2, 0, 0};
   const int size = dtype == GI_DTYPE_FP32 ? 4 : 2;
   bool vec = D % 8 == 0 && rotary_dim % (interleaved ? 8 : 16) == 0;
@@ -290,7 +292,8 @@ int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, con
   // 2047 rows of 16 + 8 heads of 256, 12.3 us)
   const int64_t parts = ((int64_t)(Hq + Hk) * a.units + kRopeThreads - 1) / kRopeThreads;
   if (parts > 65535) return fail(GI_ERR_UNSUPPORTED, "rope_rows: too many heads");
-  const dim3 grid(T, (unsigned)parts);
+  const int width = T < kRopeGrid ? T : kRopeGrid;
+  const dim3 grid(width, (unsigned)parts, (T - 1) / width + 1);
 #define GI_ROPE_V(T_, I_)                                                                                 \
   do {                                                                                                    \
     if (vec) hipLaunchKernelGGL((rope_rows_kernel<T_, I_, true>), grid, dim3(kRopeThreads), 0, stream, a);  \

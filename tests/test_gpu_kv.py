@@ -138,6 +138,25 @@ def test_rope_rows(dtype, t, hq, hk, d, rot, inter):
     assert none is None and torch.equal(only, qo)
 
 
+def test_rope_more_rows_than_a_grid_is_wide():
+    """2^24 rows and more: the last ones turn as they do in a call of their own."""
+    t, n, d = (1 << 24) + 300, 500, 16
+    freq, _ = ops.rope_frequencies(d, device=DEV)
+    q = torch.zeros(t, 1, d, dtype=BF16, device=DEV)
+    pos = torch.zeros(t, dtype=torch.int64, device=DEV)
+    own = torch.randn(n, 1, d, generator=_gen(1)).to(BF16).to(DEV)
+    ats = (0, (1 << 23) - 250, t - n)
+    for at in ats:
+        q[at:at + n] = own
+        pos[at:at + n] = torch.arange(n, device=DEV)
+    want, _ = ops.rope_rows(q[:n], None, pos[:n], freq)
+    got, _ = ops.rope_rows(q, None, pos, freq)
+    assert torch.equal(got, ops.rope_rows(q, None, pos, freq, inplace=True)[0])
+    assert not got[n:ats[1]].any() and not got[ats[1] + n:ats[2]].any()
+    for at in ats:
+        assert torch.equal(got[at:at + n], want)
+
+
 def test_rope_matches_the_table_form():
     """fused_rope_inplace with tables of the same angles: equal to a rounding of each."""
     t, d = 33, 256
