@@ -42,6 +42,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // The partial sums fit the workspace while choose_chunk's total is right to 1e-4: over this
 // many requests, 1024 to a thread, an fp32 sum is off by at most about 2^10 * 2^-24.
 constexpr int kMaxRequests = 1 << 20;
+constexpr int kMaxGrid = 1 << 23;  // workgroups: with their threads under the 2^32 that a launch may have
 // Weights go to the matrix cores in fp16 as 2^(t - m + kBias).  The reference m
 // is a maximum of earlier rows and follows when a lane's 16 weights sum to more than
 // kMostSum, so none is over 2^15; fp16 is normal down to 2^-14, so a weight
@@ -726,7 +727,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_join_kernel(AttnArgs a)
   const int hk = blockIdx.x % a.Hk;
   const int chunk = *a.plan;
   Item it;
-  if (!find_item<RT>(a, chunk, blockIdx.x / a.Hk, true, it)) return;
+  if (!find_item<RT>(a, chunk, (blockIdx.z * gridDim.x + blockIdx.x) / a.Hk, true, it)) return;
   const Span sp = span_of<RT>(a, it);
   if (it.over || sp.chunks == 1 || it.slot + sp.chunks > a.max_slots) return;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -811,7 +812,8 @@ Grid grid_of(int T, int B, int Hq, int Hk, int D, int64_t tokens) {
   // them (2056 of them 9.6 us beside one request of 1391 tokens), so there are no
   // more than it holds at a time, or tiles; each takes every so-many-th item.
   const int64_t wide = r.resident > r.max_tiles ? r.resident : r.max_tiles;
-  r.groups = (int)(most < wide ? most : wide < items ? wide : items);
+  const int64_t groups = most < wide ? most : wide < items ? wide : items;
+  r.groups = (int)(groups < kMaxGrid / Hk ? groups : kMaxGrid / Hk);
   return r;
 }
 
@@ -831,9 +833,10 @@ void launch(const AttnArgs& a, const Grid& gr, hipStream_t stream) {
   hipLaunchKernelGGL((kv_attention_kernel<D, CT, F16>), dim3(gr.groups * a.Hk), dim3(kThreads), 0, stream, a);
   // up to 2048 workgroups, each for as many of its tile's values as that leaves
   if (gr.max_slots == 0) return;
-  const int cols = (int)min((int64_t)16 * CT, (int64_t)(a.q_start ? a.T : 1) * a.G), tiles = gr.max_tiles * a.Hk;
+  const int cols = (int)min((int64_t)16 * CT, (int64_t)(a.q_start ? a.T : 1) * a.G);
+  const int per = min(gr.max_tiles, kMaxGrid / a.Hk), layers = (gr.max_tiles - 1) / per + 1, tiles = per * a.Hk;
   const int parts = min(max(2048 / tiles, 1), (cols * (D / 4) + kWave - 1) / kWave);
-  hipLaunchKernelGGL((kv_attention_join_kernel<D, CT, F16>), dim3(tiles, parts), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((kv_attention_join_kernel<D, CT, F16>), dim3(tiles, parts, layers), dim3(kThreads), 0, stream, a);
 }
 
 template <int D, bool F16>
@@ -854,7 +857,7 @@ void launch_d(const AttnArgs& a, const Grid& gr, int D, hipStream_t stream) {
 }  // namespace
 
 size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D, int64_t max_tokens) {
-  if (T <= 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || !width_ok(D) || max_tokens < 0) return 0;
+  if (T <= 0 || B <= 0 || Hk <= 0 || Hk > kMaxGrid || Hq <= 0 || Hq % Hk || !width_ok(D) || max_tokens < 0) return 0;
   return part_bytes(grid_of(T, B, Hq, Hk, D, max_tokens), B, Hk, D);
 }
 
@@ -874,6 +877,7 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
     if (page_size == 1 << l) lp = l;
   if (lp < 0) return fail(GI_ERR_INVALID_ARG, "kv_attention: page_size must be 16, 32, 64, 128 or 256");
   if (!q_start && T != B) return fail(GI_ERR_INVALID_ARG, "kv_attention: without q_start there is one row a request");
+  if (Hk > kMaxGrid) return fail(GI_ERR_UNSUPPORTED, "kv_attention: at most 2^23 kv heads");
   if (B > kMaxRequests) return fail(GI_ERR_UNSUPPORTED, "kv_attention: at most 2^20 requests");
   if (!(scale == scale)) return fail(GI_ERR_INVALID_ARG, "kv_attention: scale is NaN");
   if (window < 0) return fail(GI_ERR_INVALID_ARG, "kv_attention: window must be >= 0 (0: none)");
@@ -890,7 +894,7 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
   if (window >= (int64_t)max_pages * page_size) window = 0;  // no request is that long
   if ((uintptr_t)workspace & 15) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
   const Grid gr = grid_of(T, B, Hq, Hk, D, (int64_t)max_pages * page_size);
-  if ((int64_t)gr.groups * Hk > 0x7fffffff) return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows");
+  if ((int64_t)gr.max_tiles * Hk > 0x7fffffff) return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows");
   if (!workspace || workspace_bytes < part_bytes(gr, B, Hk, D))
     return fail(GI_ERR_WORKSPACE, "kv_attention: workspace missing or too small");
   AttnArgs a{q, q_strides[0], q_strides[1], (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale,

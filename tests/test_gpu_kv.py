@@ -491,6 +491,26 @@ def test_attention_many_requests(b):
     _check_attention([n + r for n, r in zip(lens, rows)], rows, 2, 1, 16, 64, BF16, seed=b)
 
 
+@pytest.mark.parametrize("cols", [1, 20])
+def test_attention_more_items_than_a_grid_is_wide(cols):
+    """2^18 requests on 64 kv heads (2^24 items) against the calls of their 13 x 7 x 17 kinds (row, page, length)."""
+    b, hk, d, page = 1 << 18, 64, 64, 16
+    cache = _to(_filled(7, hk, page, d, seed=1), DEV)
+    q = torch.randn(13, hk, d, generator=_gen(2)).to(BF16).to(DEV)
+    kind = torch.arange(13 * 7 * 17, device=DEV)
+    pick = torch.randint(0, len(kind), (b,), generator=_gen(3)).to(DEV)
+    pick[-len(kind):] = kind
+
+    def call(k):
+        table = torch.full((len(k), cols), -1, dtype=torch.int32, device=DEV)
+        table[:, 0] = k // 17 % 7
+        return ops.kv_attention(q[k // (17 * 7)], cache, table, (k % 17).int())
+    want = torch.cat([call(kind[i:i + 60]) for i in range(0, len(kind), 60)])
+    got = call(pick)
+    for i in range(0, b, 1 << 14):
+        assert torch.equal(got[i:i + (1 << 14)], want[pick[i:i + (1 << 14)]])
+
+
 def test_attention_long_request_among_many():
     """A request over many workgroups beside 99 short ones: its partial sums are where the join looks."""
     lens = [30] * 100

@@ -122,6 +122,15 @@ def test_largest_counts_are_refused(lib):
     assert st == L.GI_ERR_WORKSPACE
 
 
+def test_more_heads_than_a_grid_is_wide_are_refused(lib):
+    heads = (1 << 23) + 1
+    st, msg = _call(lib, "gi_kv_attention", ATTN, dict(Hq=heads, Hk=heads, q=None))
+    assert st == L.GI_ERR_UNSUPPORTED and "2^23" in msg
+    assert lib.gi_kv_attention_workspace_bytes(3, 2, heads, heads, 64, 64) == 0
+    st, msg = _call(lib, "gi_kv_attention", ATTN, dict(Hq=1 << 23, Hk=1 << 23))
+    assert st == L.GI_ERR_WORKSPACE
+
+
 def test_workspace_query_is_host_only(lib):
     q = lib.gi_kv_attention_workspace_bytes
     for bad in ((0, 1, 16, 8, 256), (1, 0, 16, 8, 256), (1, 1, 15, 8, 256), (1, 1, 16, 8, 96)):
