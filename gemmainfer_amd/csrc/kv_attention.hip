@@ -45,10 +45,14 @@ constexpr int kMaxRequests = 1 << 20;
 constexpr int kMaxGrid = 1 << 23;  // workgroups: with their threads under the 2^32 that a launch may have
 // Weights go to the matrix cores in fp16 as 2^(t - m + kBias).  The reference m
 // is a maximum of earlier rows and follows when a lane's 16 weights sum to more than
-// kMostSum, so none is over 2^15; fp16 is normal down to 2^-14, so a weight
-// 2^-17 of that of m still has all 11 bits, and a lighter one is off by at most 2^-28 of it.
-constexpr float kBias = 3.f;
-constexpr float kMostSum = 32768.f;
+// kMostSum, so none is over fp16's largest; fp16 is normal down to 2^-14, so a weight
+// 2^-25 of that of m still has all 11 bits, and a lighter one is off by at most 2^-36 of
+// it: a flat tail behind one heavy token loses less than half a step of fp16 (2^-11)
+// over 2^25 tokens.  With a bias of 3 (2^-28) the sums could grow 2^8 times as much
+// before the reference follows: 2048 rows on 8100 tokens 272 instead of 285 us where
+// scores are spread widely (deviation 6), 274 instead of 266 where they are not (1.5).
+constexpr float kBias = 11.f;
+constexpr float kMostSum = 65504.f;
 
 struct AttnArgs {
   const void* q;

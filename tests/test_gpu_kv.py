@@ -532,6 +532,44 @@ def test_attention_peaked_and_flat(window):
         _check_attention([500, 77], [5, 3], 4, 2, 16, 128, FP16, window, seed=3, scale=scale, q_size=size)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("at", [0, 5, 4000, 8191])
+def test_attention_flat_tail_behind_a_heavy_token(dtype, at):
+    """One token of 2^30 times the weight of each of 8191 others, with values of its own in half the
+    dimensions only: what the others add up to in the rest is seen.  Forty requests, so that a
+    request is not cut into chunks, and a wave meets a quarter of it."""
+    hk, d, n, b, page = 64, 64, 8192, 40, 64
+    g = _gen(at)
+    k, v = torch.zeros(n, hk, d), 0.5 + 0.5 * torch.rand(n, hk, d, generator=g)
+    k[..., 0] = 2 * torch.rand(n, hk, generator=g) - 1
+    k[at, :, 0] = 30.0
+    v[at, :, :32], v[at, :, 32:] = 1.5, 0.0
+    k, v = k.to(O.E4M3), v.to(O.E4M3)
+    ones = torch.ones(n // page, hk)
+    cache = ops.KVCache(k.view(n // page, page, hk, d).transpose(1, 2).contiguous(),
+                        v.view(n // page, page, hk, d).permute(0, 2, 3, 1).contiguous(), ones, ones)
+    q = torch.zeros(b, hk, d)
+    q[..., 0] = 16 * torch.exp2(-torch.rand(b, 1, generator=g) / 16)
+    q[..., 1:] = torch.randn(b, hk, d - 1, generator=g)
+    q = q.to(dtype)
+    scale = 0.6931471805599453 / 16
+    got = ops.kv_attention(q.to(DEV), _to(cache, DEV), _i32([list(range(n // page))] * b), _i32([n] * b), scale=scale)
+    ref, weighted = torch.zeros(b, hk, d, dtype=torch.float64), torch.zeros(b, hk, d, dtype=torch.float64)
+    for h in range(hk):
+        p = torch.softmax(q[:, h].double() @ k[:, h].double().t() * scale, -1)
+        ref[:, h] = weighted[:, h] = p @ v[:, h].double()  # no value is negative
+    # as in _check_out, with weights of 2^11 times their share (65504 at most, so the heaviest is 2^11 or more):
+    # half a step is 2^-11 of one over 2^-25 of the heaviest, below that 2^-36 of the heaviest, and as much
+    # again where the heaviest is up to twice the reference
+    e = (d + 8) * 2.0 ** -24 * (30 * 0.6931471805599453 + 28)
+    w = 2.0 ** -11 + 2 * e + 2 * n * 2.0 ** -24
+    bound = (HALF[dtype] * ref + (1 + HALF[dtype]) * w * weighted + n * 2.0 ** -35 * float(v.float().max())
+             + (2.0 ** -24 if dtype == FP16 else 0.0))
+    err = (got.cpu().double() - ref).abs()
+    assert (err <= bound).all(), (err / bound).max()
+    assert (ref[..., 32:] > 4e-6).all()
+
+
 def _poison_rest(cache, table, lens):
     """Everything of the cache that no request holds: NaN codes; scales of unused pages NaN."""
     page = cache.k.shape[2]
