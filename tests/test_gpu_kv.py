@@ -311,6 +311,32 @@ def test_append_holes_of_any_length(hk, hole):
         _check_append(cache, k, v, slots)
 
 
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("t,hk", [(1040, 8), (300, 40), (9000, 1)])
+def test_append_many_pages_a_workgroup(t, hk, page):
+    """More than 8192 rows of heads, as of a large decode step: lone rows on pages of their own, then
+    runs of 3 to 7, whole pages, and skipped rows, so that a workgroup's sixteen rows are many runs."""
+    rng = random.Random(t)
+    pages = t
+    cache = _filled(1, 2, page, 8, seed=t)
+    scale = torch.exp2(torch.randint(-8, 3, (2, pages, hk), generator=_gen(t)).float())
+    cache = ops.KVCache(cache.k.view(torch.uint8)[:, :1].expand(pages, hk, page, 8).contiguous().view(O.E4M3),
+                        cache.v.view(torch.uint8)[:, 1:].expand(pages, hk, 8, page).contiguous().view(O.E4M3),
+                        scale[0].contiguous(), scale[1].contiguous())
+    for runs in ([1], [1, 3, 7, 4], [1, 2, 5, page, 2 * page]):
+        ids = list(range(pages))
+        rng.shuffle(ids)
+        slots = []
+        while len(slots) < t:
+            n, p = rng.choice(runs), ids.pop()
+            first = rng.randrange(page)
+            slots += [p * page + (first + i) % page for i in range(n)]
+            if rng.random() < 0.2:
+                slots.append(rng.choice([-1, pages * page + 5]))
+        k, v = _sized_rows(t, hk, 8, t)
+        _check_append(cache, k, v, slots[:t])
+
+
 @pytest.mark.parametrize("page,hk,t", [(16, 2, 900), (16, 40, 900), (64, 40, 2000), (256, 33, 1500)])
 def test_append_random_runs_and_holes(page, hk, t):
     """Pages in any order, runs of 1 to 40 rows in any order of places (some named twice), holes of
@@ -523,6 +549,33 @@ def test_attention_long_request_among_many():
 def test_attention_long_axis_is_cut_and_joined(hq, hk, d, rows):
     """A context over many workgroups: their partial sums, with sizes that differ from page to page."""
     _check_attention([9001], [rows], hq, hk, 64, d, BF16, seed=rows, spread=3.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("hq,hk,d,page", [(16, 8, 256, 16), (16, 2, 512, 64), (4, 4, 64, 16), (8, 1, 128, 128)])
+@pytest.mark.parametrize("window", [512, 1024, 1500])
+@pytest.mark.parametrize("lens,rows", [([9000, 1500, 511, 1023], [1, 1, 1, 1]),        # decode
+                                       ([1500, 4001, 600, 1030], [7, 1, 5, 7]),        # verify
+                                       ([1100, 3000, 40], [130, 33, 40])])             # prompts over the window's end
+def test_attention_windowed_requests_are_cut(dtype, hq, hk, d, page, window, lens, rows):
+    """Windows of several chunks that start inside the request: partial sums, and the chunks that a
+    tile of the list has and its window does not."""
+    _check_attention(lens, rows, hq, hk, page, d, dtype, window, seed=window + sum(rows), spread=2.0)
+
+
+@pytest.mark.parametrize("b", [65, 130])
+@pytest.mark.parametrize("hq,hk,d,rows", [(8, 2, 64, 6), (8, 2, 64, 12), (16, 8, 256, 9), (16, 8, 256, 17), (16, 2, 512, 3)])
+@pytest.mark.parametrize("window", [0, 512])
+def test_attention_many_requests_of_many_rows(b, hq, hk, d, rows, window):
+    """The plan of more than 64 requests with tiles of 32 and 64 columns, one request cut and joined,
+    some without rows or tokens."""
+    rng = random.Random(b * rows)
+    counts = [rng.choice([rows, rows, rows, 2 * rows, 1, 0]) for _ in range(b)]
+    while sum(counts) < (rows - 1) * b:  # the mean decides the tile
+        counts[rng.randrange(b)] = 2 * rows
+    lens = [max(0, n + rng.choice([-1, 0, 0, 5, 60])) for n in counts]
+    lens[b // 2], counts[b // 2] = 4000, rows
+    _check_attention(lens, counts, hq, hk, 16, d, BF16, window, seed=b + rows, spread=2.0)
 
 
 @pytest.mark.parametrize("window", [0, 50])
