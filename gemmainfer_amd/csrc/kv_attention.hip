@@ -617,7 +617,10 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
       // ---- O^T += V^T P^T
       // (masked in every unit: one straight line of code is scheduled better than two, 3% of the
       // instructions of 64 columns)
-      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+      // a page that is not there, or has no scale: its rows weigh NaN where they are seen and nothing where
+      // they are not, and what was read in its place may hold anything
+      const uint32_t all = cur.vs == cur.vs ? ~0u : 0u;
+      uint32_t keep[4] = {all, all, all, all};
       if (edge) {  // rows that no column sees may hold anything
         const int last = min(pos_max - (tok + 16 * g), 15);
         const int first = a.window > 0 ? pos_min - a.window + 1 - (tok + 16 * g) : 0;
@@ -626,7 +629,7 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
           keep[x] = 0;
 #pragma unroll
           for (int y = 0; y < 4; ++y)
-            if (4 * x + y <= last && 4 * x + y >= first) keep[x] |= 0xffu << (8 * y);
+            if (4 * x + y <= last && 4 * x + y >= first) keep[x] |= all & 0xffu << (8 * y);
         }
       }
 #pragma unroll

@@ -695,6 +695,31 @@ def test_attention_missing_pages_and_poisoned_scales_give_nan():
     assert (got == 0).all()
 
 
+@pytest.mark.parametrize("hq,d,page", [(4, 64, 16), (4, 256, 16), (4, 512, 64), (20, 128, 32)])
+def test_attention_missing_pages_spare_earlier_rows_whatever_the_pool_holds(hq, d, page):
+    """Rows in front of a missing page, in a tile with rows behind it, in a pool whose unheld places
+    are NaN codes (a pool that was not zeroed)."""
+    lens, rows = [200, 150], [90, 40]
+    cache, table, start = _setup(lens, rows, 2, page, d, seed=3)
+    free = [p for p in range(cache.k.shape[0]) if not any(p in r for r in table)]
+    q = torch.randn(start[-1], hq, d, generator=_gen(4)).to(BF16).to(DEV)
+    clean = ops.kv_attention(q, _to(cache, DEV), _i32(table), _i32(lens), _i32(start))
+    _poison_rest(cache, table, lens)
+    move = [free[0], *[p for p in range(cache.k.shape[0]) if p != free[0]]]  # page 0 is one that no request holds
+    at = {old: new for new, old in enumerate(move)}
+    cache = ops.KVCache(*[(x.view(torch.uint8)[move].view(x.dtype) if x.dtype == O.E4M3 else x[move]) for x in cache])
+    cache.k_scale[0] = cache.v_scale[0] = 1.0
+    table = [[at.get(p, -1) for p in r] for r in table]
+    table[0][128 // page] = -1                 # tokens 128 to 128 + page
+    table[1][128 // page] = cache.k.shape[0]
+    got = ops.kv_attention(q, _to(cache, DEV), _i32(table), _i32(lens), _i32(start))
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[128 - 110:90] = True
+    bad[90 + 128 - 110:] = True
+    assert torch.equal(torch.isnan(got), bad)
+    assert torch.equal(got[~bad], clean[~bad])
+
+
 @pytest.mark.parametrize("window", [2 ** 31 - 1, 64, 63])
 def test_attention_windows_around_the_table(window):
     """Windows as long as the table and longer, with rows that see nothing beside ones that do."""
