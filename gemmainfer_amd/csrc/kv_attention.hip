@@ -269,6 +269,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int chunk, int want
     in = want - (by_tile ? before.y : before.x);
     slot = before.z;
     l = load_of<RT>(a, it.b);
+    // requests that share rows (offsets that decrease) can be more than the counts hold
+    if (in < 0 || in >= l.tiles * (by_tile ? 1 : max(ceil_div(l.units, chunk), 1))) return false;
   }
   const int per = max(ceil_div(l.units, chunk), 1);
   const int tile = by_tile ? in : in / per;
@@ -423,7 +425,9 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
   for (int want = blockIdx.x / a.Hk; find_item<RT>(a, chunk, want, false, it); want += gridDim.x / a.Hk) {
   const Span sp = span_of<RT>(a, it);
   const int r0 = it.tile * RT, n_cols = min(RT, it.rows * a.G - r0);
-  if (it.over) {
+  // longer than the table, or (which choose_chunk's total rules out) without room for its partial sums
+  const bool lost = it.over || (sp.chunks > 1 && it.slot + sp.chunks > a.max_slots);
+  if (lost) {
     if (it.chunk_no == 0) {
       const uint32_t nan = F16 ? 0x7e007e00u : 0x7fc07fc0u;
       for (int e = threadIdx.x; e < n_cols * (D / 8); e += kThreads) {
@@ -434,7 +438,7 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
     }
     continue;
   }
-  if (it.chunk_no >= sp.chunks || (sp.chunks > 1 && it.slot + sp.chunks > a.max_slots)) continue;
+  if (it.chunk_no >= sp.chunks) continue;
   __syncthreads();  // the item before is done with LDS
   const int lane = this_lane();
   const int i16 = lane & 15, g = lane >> 4;

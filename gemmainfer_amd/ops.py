@@ -817,14 +817,15 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
     """Causal attention of packed query rows q [T, Hq, D] (bf16 or fp16) over the
     cache; returns [T, Hq, D].
 
-    Rows ``q_start[b]`` to ``q_start[b + 1]`` (int32 [B + 1]; None: one row a
-    request) are the last tokens of request b, which has ``seq_lens[b]`` (int32)
+    Rows ``q_start[b]`` to ``q_start[b + 1]`` (int32 [B + 1], which must not
+    decrease; None: one row a request) are the last tokens of request b, which has ``seq_lens[b]`` (int32)
     tokens in the pages ``block_table[b]`` names, those rows' own among them.  A
     row sees the tokens up to its own, with ``window`` > 0 the last ``window`` of
     them; one that sees none gets zeros.  ``scale`` defaults to D ** -0.5.  Query
     head h reads kv head h // (Hq // Hk).  Rows behind the last request are not
     computed: they keep what ``out`` holds, and are unspecified without it.  A
-    row that sees a token without a page (outside the cache, or past the table) gets NaN."""
+    row that sees a token without a page (one outside the cache) gets NaN, and so
+    does every row of a request that is longer than its table."""
     if q_start is None:
         dev = _on_device(q, block_table, seq_lens, *cache)
     else:

@@ -409,8 +409,8 @@ int gi_kv_append(const void* k, const void* v, int dtype,
                  void* k_cache, void* v_cache, float* k_scale, float* v_scale, void* stream);
 
 /* out[t, h] = softmax(scale * q[t, h] . K) V over the tokens that row t sees.
- * Rows q_start[b] ... q_start[b+1]-1 belong to request b (NULL: one row a
- * request, T == B) and are its last ones: with n rows, row i is at position
+ * Rows q_start[b] ... q_start[b+1]-1 belong to request b (q_start must not
+ * decrease; NULL: one row a request, T == B) and are its last ones: with n rows, row i is at position
  * seq_lens[b] - n + i and sees tokens up to it, and with window > 0 only the
  * last `window` of those.  Head h reads kv head h / (Hq / Hk).  A row that
  * sees nothing gets zeros; rows behind q_start[B] are not touched.  A row that
