@@ -791,6 +791,7 @@ int after_launch(const char* what) {
   return e == hipSuccess ? GI_OK : hip_fail(e, what);
 }
 
+// Tiles of 16 columns, by the mean columns of a request.
 int col_tiles(int T, int B, int G, int D) {
   const int64_t rows = ((int64_t)T * G + B - 1) / B;
   if (rows <= 16) return 1;
@@ -802,21 +803,21 @@ struct Grid {
   int ct, resident, max_tiles, max_slots, groups;
 };
 
-Grid grid_of(int T, int B, int Hq, int Hk, int D, int64_t tokens) {
+Grid grid_of(int T, int B, int Hq, int Hk, int D, int64_t tokens, int ct) {
   const int G = Hq / Hk;
   Grid r;
-  r.ct = col_tiles(T, B, G, D);
+  r.ct = ct;
   const int RT = 16 * r.ct;
   const int64_t cols = (int64_t)T * G;
   // a request's last tile may be cut: ceil(rows * G / RT) tiles
   r.max_tiles = (int)(cols < cols / RT + B ? cols : cols / RT + B);
   r.resident = (workgroups_per_cu(D, r.ct) * 256 + Hk - 1) / Hk;
   // chunk >= total / (kRounds * resident), so the chunks of all tiles are at
-  // most kRounds * resident and one more for each; those of tiles that are cut
-  // (units > chunk) at most twice as many as total / chunk, nor more than the longest table has
+  // most kRounds * resident and one more for each; of tiles that are cut (units >
+  // chunk) there are at most total / chunk, and no more chunks than the longest table has
   const int64_t per_tile = (tokens / kUnit + 1 + kMinChunk - 1) / kMinChunk;
   const int64_t items = kRounds * (int64_t)r.resident + r.max_tiles;
-  const int64_t slots = 2 * kRounds * (int64_t)r.resident;
+  const int64_t slots = items < 2 * kRounds * (int64_t)r.resident ? items : 2 * kRounds * (int64_t)r.resident;
   const int64_t most = r.max_tiles * per_tile;
   r.max_slots = (int)(tokens <= kMinChunk * kUnit ? 0 : most < slots ? most : slots);
   // Workgroups without an item cost a round of the chip each time it is full of
@@ -869,7 +870,17 @@ void launch_d(const AttnArgs& a, const Grid& gr, int D, hipStream_t stream) {
 
 size_t kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D, int64_t max_tokens) {
   if (T <= 0 || B <= 0 || Hk <= 0 || Hk > kMaxGrid || Hq <= 0 || Hq % Hk || !width_ok(D) || max_tokens < 0) return 0;
-  return part_bytes(grid_of(T, B, Hq, Hk, D, max_tokens), B, Hk, D);
+  // Fewer requests can mean wider tiles and more to hold: the most that any call of up to T rows and B
+  // requests needs, width by width (the wider ones are of calls with few requests).
+  const int64_t cols = (int64_t)T * (Hq / Hk);
+  size_t need = 0;
+  for (int ct = 1; ct <= col_tiles(T, 1, Hq / Hk, D); ct *= 2) {
+    const int64_t most = ct == 1 ? B : (cols - 1) / (8 * ct);  // (cols + b - 1) / b > 8 ct
+    const Grid gr = grid_of(T, (int)(most < B ? most : B), Hq, Hk, D, max_tokens, ct);
+    const size_t bytes = part_bytes(gr, B, Hk, D);
+    need = need > bytes ? need : bytes;
+  }
+  return need;
 }
 
 int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, const void* k_cache, const void* v_cache,
@@ -904,7 +915,7 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
     if (s % 8) return fail(GI_ERR_INVALID_ARG, "kv_attention: row and head strides must be multiples of 8 elements");
   if (window >= (int64_t)max_pages * page_size) window = 0;  // no request is that long
   if ((uintptr_t)workspace & 15) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
-  const Grid gr = grid_of(T, B, Hq, Hk, D, (int64_t)max_pages * page_size);
+  const Grid gr = grid_of(T, B, Hq, Hk, D, (int64_t)max_pages * page_size, col_tiles(T, B, Hq / Hk, D));
   if ((int64_t)gr.max_tiles * Hk > 0x7fffffff) return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows");
   if (!workspace || workspace_bytes < part_bytes(gr, B, Hk, D))
     return fail(GI_ERR_WORKSPACE, "kv_attention: workspace missing or too small");

@@ -420,7 +420,9 @@ int gi_kv_append(const void* k, const void* v, int dtype,
  * multiples of 8 elements, 16-byte aligned; D 64, 128, 256 or 512; fp32 sums
  * and softmax statistics.  Deterministic.  The workspace is scratch: it needs
  * no initial value and holds nothing between calls.  Its size depends on
- * max_tokens = max_pages * page_size, what a row of the table has room for. */
+ * max_tokens = max_pages * page_size, what a row of the table has room for, and
+ * does not shrink as T, B or max_tokens grow: a workspace for a program's largest
+ * numbers serves its smaller calls on the same heads.                       */
 size_t gi_kv_attention_workspace_bytes(int T, int B, int Hq, int Hk, int D, int64_t max_tokens);
 int gi_kv_attention(const void* q, int dtype, int64_t q_st, int64_t q_sh,
                     const void* k_cache, const void* v_cache,

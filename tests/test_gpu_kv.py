@@ -578,6 +578,52 @@ def test_attention_many_requests_of_many_rows(b, hq, hk, d, rows, window):
     _check_attention(lens, counts, hq, hk, 16, d, BF16, window, seed=b + rows, spread=2.0)
 
 
+@pytest.mark.parametrize("hq,hk,d", [(16, 8, 256), (16, 2, 512), (12, 4, 64)])
+def test_attention_on_one_workspace(hq, hk, d):
+    """The C entry with a workspace for 64 rows of 64 requests: every smaller call is served by it,
+    with the bits of a call with its own, and nothing behind it is written."""
+    lib, page, n = L.load(), 16, 2000
+    cols = n // page
+    cache = _to(_filled(cols, hk, page, d, seed=1), DEV)
+    table = _i32([list(range(cols))] * 64)
+    nbytes = lib.gi_kv_attention_workspace_bytes(64, 64, hq, hk, d, n)
+    for t, b in ((64, 64), (64, 1), (64, 2), (64, 3), (64, 4), (64, 9), (40, 2), (17, 1), (9, 1), (1, 1), (5, 64)):
+        q = torch.randn(t, hq, d, generator=_gen(t)).to(BF16).to(DEV)
+        start = _i32([min(i * -(-t // b), t) for i in range(b + 1)])
+        lens = _i32([n - 37 * i % 900 for i in range(b)])
+        want = ops.kv_attention(q, cache, table[:b], lens, start)
+        ws = torch.full((nbytes + 4096,), 0xAB, dtype=torch.uint8, device=DEV)
+        out = torch.zeros_like(q)
+        st = lib.gi_kv_attention(q.data_ptr(), L.DTYPE_BF16, hq * d, d, *[x.data_ptr() for x in cache], table.data_ptr(),
+                                 cols, cols, lens.data_ptr(), start.data_ptr(), out.data_ptr(), hq * d, d, t, b, hq, hk,
+                                 d, page, cols, d ** -0.5, 0, ws.data_ptr(), nbytes,
+                                 torch.cuda.current_stream().cuda_stream)
+        assert st == L.GI_OK, (t, b, lib.gi_last_error())
+        assert torch.equal(out, want) and (ws[nbytes:] == 0xAB).all(), (t, b)
+
+
+@pytest.mark.parametrize("hk,d,g", [(1, 64, 3), (8, 64, 2), (2, 128, 4), (8, 256, 2), (2, 512, 8)])
+def test_attention_partial_sums_have_room(hk, d, g):
+    """Batches whose lengths and rows differ by powers of two: no tile is without room for its chunks
+    (it would be NaN)."""
+    rng = random.Random(d + hk)
+    page, cols = 64, 400
+    cache = _to(_filled(8, hk, page, d, seed=1), DEV)
+    cache = ops.KVCache(*[x[torch.arange(cols, device=DEV) % 8] if x.dtype == FP32 else
+                          x.view(torch.uint8)[torch.arange(cols, device=DEV) % 8].view(x.dtype) for x in cache])
+    for _ in range(40):
+        b = rng.choice([1, 2, 5, 20, 64, 65, 150])
+        rows = [int(2 ** rng.uniform(0, rng.choice([0, 3, 6]))) for _ in range(b)]
+        lens = [r + int(2 ** rng.uniform(0, rng.choice([6, 10, 14.5]))) for r in rows]
+        start = [0]
+        for r in rows:
+            start.append(start[-1] + r)
+        q = torch.randn(start[-1], hk * g, d, generator=_gen(b)).to(BF16).to(DEV)
+        got = ops.kv_attention(q, cache, _i32([list(range(cols))] * b), _i32(lens), _i32(start),
+                               window=rng.choice([0, 0, 700]))
+        assert torch.isfinite(got).all(), (rows, lens)
+
+
 @pytest.mark.parametrize("window", [0, 50])
 def test_attention_peaked_and_flat(window):
     """Weights of one token, scores that run away late, and a scale of 0 (plain means)."""

@@ -140,6 +140,18 @@ def test_workspace_query_is_host_only(lib):
     assert q(64, 64, 16, 8, 256, 1 << 20) < 1 << 27    # bounded by what the chip holds, not by the lengths
 
 
+@pytest.mark.parametrize("hq,hk,d", [(16, 8, 256), (16, 2, 512), (32, 8, 128), (12, 4, 64), (40, 1, 64), (64, 64, 64)])
+def test_workspace_query_does_not_shrink(lib, hq, hk, d):
+    """One workspace for the largest T, B and table serves every smaller call."""
+    q = lib.gi_kv_attention_workspace_bytes
+    sizes = [1, 2, 3, 7, 16, 17, 33, 64, 65, 100, 512, 4000]
+    for tokens in (256, 272, 4096, 1 << 17):
+        need = {(t, b): q(t, b, hq, hk, d, tokens) for t in sizes for b in sizes}
+        for (t, b), n in need.items():
+            assert n >= max(need[x, y] for x in sizes if x <= t for y in sizes if y <= b), (t, b, tokens)
+            assert n <= q(t, b, hq, hk, d, 2 * tokens)
+
+
 def test_device_calls_reject_host_tensors():
     x = torch.zeros(1, 1, 64, dtype=torch.bfloat16)
     i = torch.zeros(1, dtype=torch.int64)
