@@ -847,6 +847,7 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
         raise ValueError(f"kv_attention: without q_start there is one row a request: {t} rows, {b} requests")
     if window < 0:
         raise ValueError(f"kv_attention: window must be >= 0 (0: none), got {window}")
+    window = min(window, 0x7fffffff)  # what the C entry's int holds; no table is that long
     if out is None:
         out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
         os = (hq * d, d)

@@ -669,6 +669,15 @@ def test_attention_flat_tail_behind_a_heavy_token(dtype, at):
     assert (ref[..., 32:] > 4e-6).all()
 
 
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 63 - 1, 2 ** 70])
+def test_attention_windows_past_32_bits(window):
+    """Longer than any table: no window, not what its low 32 bits say."""
+    cache, table, start = _setup([90], [7], 1, 16, 64, seed=5)
+    q = torch.randn(7, 2, 64, generator=_gen(4)).to(BF16).to(DEV)
+    args = (q, _to(cache, DEV), _i32(table), _i32([90]), _i32(start))
+    assert torch.equal(ops.kv_attention(*args, window=window), ops.kv_attention(*args))
+
+
 def _poison_rest(cache, table, lens):
     """Everything of the cache that no request holds: NaN codes; scales of unused pages NaN."""
     page = cache.k.shape[2]
