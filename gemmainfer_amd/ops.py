@@ -588,6 +588,7 @@ class KVSlots(NamedTuple):
 _PAGE_SIZES = (16, 32, 64, 128, 256)
 _HEAD_WIDTHS = (64, 128, 256, 512)
 _ROW_DTYPES = (torch.bfloat16, torch.float16)
+_MAX_COUNT = 0x7fffffff  # rows, requests and table columns are ints of the C entries
 
 
 # A decode step calls these a few times a layer with kernels of microseconds:
@@ -641,6 +642,8 @@ def _vector(t, dtype, who, name, numel=None):
         raise TypeError(f"{who}: {name} must be {dtype}, got {t.dtype}")
     if t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{who}: {name} must be a contiguous vector")
+    if t.numel() > _MAX_COUNT:
+        raise ValueError(f"{who}: {name} must have fewer than 2^31 elements, got {t.numel()}")
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{who}: {name} must have {numel} elements, got {t.numel()}")
 
@@ -651,6 +654,8 @@ def _table(block_table, batch, who):
     if block_table.dim() != 2 or block_table.shape[0] != batch:
         raise ValueError(f"{who}: block_table must be [B={batch}, pages], got {tuple(block_table.shape)}")
     cols, (rs, cs) = block_table.shape[1], block_table.stride()
+    if cols > _MAX_COUNT:
+        raise ValueError(f"{who}: block_table must have fewer than 2^31 columns, got {cols}")
     if cols > 1 and cs != 1:
         raise ValueError(f"{who}: block_table's rows must be contiguous")
     if batch > 1 and rs < cols:
@@ -838,6 +843,8 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
     if d not in _HEAD_WIDTHS:
         raise ValueError(f"kv_attention: head width must be one of {_HEAD_WIDTHS}, got {d}")
     t, hq, _ = q.shape
+    if t > _MAX_COUNT:
+        raise ValueError(f"kv_attention: fewer than 2^31 rows, got {t}")
     b = seq_lens.numel()
     _vector(seq_lens, torch.int32, "kv_attention", "seq_lens")
     cols, stride = _table(block_table, b, "kv_attention")
@@ -847,7 +854,7 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
         raise ValueError(f"kv_attention: without q_start there is one row a request: {t} rows, {b} requests")
     if window < 0:
         raise ValueError(f"kv_attention: window must be >= 0 (0: none), got {window}")
-    window = min(window, 0x7fffffff)  # what the C entry's int holds; no table is that long
+    window = min(window, _MAX_COUNT)  # what the C entry's int holds; no table is that long
     if out is None:
         out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
         os = (hq * d, d)

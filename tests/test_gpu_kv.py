@@ -936,6 +936,31 @@ def test_steps_of_a_layer_in_two_graphs():
 # ---------------------------------------------------------------------------
 # refusals of the torch-facing calls
 # ---------------------------------------------------------------------------
+def test_counts_past_31_bits_are_refused():
+    """Not served as what their low 32 bits say."""
+    n = 2 ** 32 + 3
+    cache = ops.kv_cache(4, 2, 16, 64, DEV)
+    row = torch.zeros(1, 2, 64, dtype=BF16, device=DEV)
+    slots = torch.empty(n, dtype=torch.int64, device=DEV)
+    ints = slots.view(torch.int32)[:n]
+    one, table = _i32([1]), _i32([[0, 1]])
+    freq = ops.rope_frequencies(64, device=DEV)[0]
+    calls = [
+        lambda: ops.kv_append(row.expand(n, 2, 64), row.expand(n, 2, 64), slots, cache),
+        lambda: ops.rope_rows(row.expand(n, 2, 64), None, slots, freq),
+        lambda: ops.kv_slots(one, one, table, ints, one, 16, 3),
+        lambda: ops.kv_slots(one, one, ints[None], one, one, 16, 3),
+        lambda: ops.kv_slots(ints, ints, table.expand(n, 2), one, one, 16, 3),
+        lambda: ops.kv_attention(row.expand(n, 2, 64), cache, table, one, _i32([0, 1])),
+        lambda: ops.kv_attention(row, cache, ints[None], one),
+        lambda: ops.kv_attention(row.expand(n, 2, 64), cache, table.expand(n, 2), ints),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
+            print("no refusal of call", i)
+
+
 def test_refusals():
     cache = ops.kv_cache(4, 2, 16, 64, DEV)
     x = torch.zeros(3, 2, 64, dtype=BF16, device=DEV)
