@@ -730,7 +730,7 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optiona
 def rope_rows(q, k, positions, inv_freq, *, interleaved: bool = False, mscale: float = 1.0, inplace: bool = False):
     """Rotary embedding of packed rows q [T, Hq, D] and k [T, Hk, D] (or None) at
     ``positions`` (int64 [T]); returns the rotated (q, k), which are q and k
-    themselves with ``inplace``.
+    themselves with ``inplace`` (they must not share elements then).
 
     ``inv_freq`` (fp64, on the device; ``rope_frequencies``) holds one frequency
     per rotated pair: the first 2 * len(inv_freq) dimensions turn, pair i being
@@ -760,8 +760,10 @@ def rope_rows(q, k, positions, inv_freq, *, interleaved: bool = False, mscale: f
     if inplace:
         qo, ko, qos, kos = q, k, qs, ks
         for name, x in (("q", q), ("k", k)):
-            if x is not None and any(st == 0 and n > 1 for st, n in zip(x.stride(), x.shape)):
+            if x is not None and _broadcast(x):
                 raise ValueError(f"rope_rows: {name} has broadcast dimensions, which cannot be rotated in place")
+        if k is not None and k.data_ptr() == q.data_ptr() and k.numel() and q.numel():
+            raise ValueError("rope_rows: q and k are the same elements, which cannot both be rotated in place")
     else:
         qo = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
         qos = (hq * d, d)
@@ -807,6 +809,10 @@ def kv_append(k, v, slots, cache: KVCache) -> None:
 def _rows_aligned(x):
     s = x.stride()
     return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and x.data_ptr() % 16 == 0
+
+
+def _broadcast(x):
+    return any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape))
 
 
 def _overlap(x, y):
@@ -864,6 +870,8 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
             raise ValueError("kv_attention: out must be like q, its rows contiguous and 16-byte aligned")
         if _overlap(q, out):
             raise ValueError("kv_attention: out must not overlap q")
+        if _broadcast(out):
+            raise ValueError("kv_attention: out has broadcast dimensions, whose rows would be written together")
         os = out.stride()
     if t == 0 or b == 0:
         return out

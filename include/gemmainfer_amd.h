@@ -356,7 +356,8 @@ int gi_rope_inplace(void* q, void* k, const void* cos_t, const void* sin_t,
 
 /* Rotary embedding of packed rows: q [T, Hq, D], k [T, Hk, D] (k may be NULL),
  * last dimension contiguous, row/head strides in elements, into q_out/k_out
- * (which may be q/k with the same strides: in place).  Pair i of the first
+ * (which may be q/k with the same strides: in place; results must share no
+ * elements otherwise, with each other or with an input).  Pair i of the first
  * rotary_dim dimensions, (i, i + rotary_dim/2) or, interleaved, (2i, 2i+1),
  * turns by positions[t] * inv_freq[i]; the angle is formed and reduced in fp64.
  * mscale multiplies cos and sin (1 unless the frequencies are scaled for long

@@ -936,6 +936,24 @@ def test_steps_of_a_layer_in_two_graphs():
 # ---------------------------------------------------------------------------
 # refusals of the torch-facing calls
 # ---------------------------------------------------------------------------
+def test_results_that_share_elements_are_refused():
+    """Rows or heads of a result on the same memory would be written by several workgroups at once."""
+    cache = ops.kv_cache(4, 2, 16, 64, DEV)
+    q = torch.zeros(3, 4, 64, dtype=BF16, device=DEV)
+    t, n, s = _i32([[0, 1]] * 3), _i32([1, 2, 3]), torch.zeros(3, dtype=torch.int64, device=DEV)
+    freq = ops.rope_frequencies(64, device=DEV)[0]
+    for out in (torch.zeros_like(q[:1]).expand(3, 4, 64), torch.zeros_like(q[:, :1]).expand(3, 4, 64)):
+        with pytest.raises(ValueError, match="broadcast"):
+            ops.kv_attention(q, cache, t, n, out=out)
+    one = torch.zeros(3, 4, 64, dtype=BF16, device=DEV).transpose(0, 1)[:, :1].transpose(0, 1)  # a single row of any stride
+    assert ops.kv_attention(q[:1], cache, t[:1], n[:1], out=one) is one
+    for k in (q, q[:, :2]):
+        with pytest.raises(ValueError, match="same elements"):
+            ops.rope_rows(q, k, s, freq, inplace=True)
+        ops.rope_rows(q, k, s, freq)
+    ops.rope_rows(q[:, :3], q[:, 3:], s, freq, inplace=True)
+
+
 def test_counts_past_31_bits_are_refused():
     """Not served as what their low 32 bits say."""
     n = 2 ** 32 + 3
