@@ -706,7 +706,8 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: Optiona
       frequency and divides the slowest by ``factor``;
     * ``scaling="yarn"``: frequencies that turn more than ``fast`` times in
       ``original_len`` tokens are left, those of fewer than ``slow`` turns are
-      divided by ``factor``, with a linear ramp over the turns between; mscale = 0.1 ln(factor) + 1.
+      divided by ``factor``, with a linear ramp over the turns between (over the turns, not
+      over the frequency's index); mscale = 0.1 ln(factor) + 1.
     """
     _require(rotary_dim > 0 and rotary_dim % 2 == 0, f"rope_frequencies: rotary_dim must be even, got {rotary_dim}")
     _require(scaling in (None, "linear", "ntk", "yarn"),

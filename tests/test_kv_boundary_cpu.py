@@ -1,6 +1,7 @@
 """Host-side argument checks of the paged-cache entry points (they return before any HIP call),
 and the oracle's own rounding."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -159,6 +160,24 @@ def test_device_calls_reject_host_tensors():
         ops.rope_rows(x, None, i, torch.zeros(32, dtype=torch.float64))
     with pytest.raises(TypeError, match="device tensors"):
         ops.kv_append(x, x, i, ops.kv_cache(1, 1, 16, 64, "cpu"))
+
+
+@pytest.mark.parametrize("rotary,base,factor,original,fast,slow", [
+    (128, 1e4, 16.0, 8192, 32.0, 1.0), (64, 5e5, 4.0, 4096, 32.0, 1.0), (256, 1e6, 40.0, 32768, 64.0, 2.0),
+    (16, 1e4, 2.0, 100, 3.0, 0.5)])
+def test_yarn_ramp_is_linear_in_the_turns(rotary, base, factor, original, fast, slow):
+    """Every frequency, one at a time: kept over `fast` turns in `original` tokens, divided by `factor` under
+    `slow`, and between them the share (turns - slow) / (fast - slow) of it is kept."""
+    got, mscale = ops.rope_frequencies(rotary, base, scaling="yarn", factor=factor, original_len=original, fast=fast,
+                                       slow=slow, device="cpu")
+    seen = set()
+    for i in range(rotary // 2):
+        f = base ** (-2.0 * i / rotary)
+        turns = original * f / (2 * math.pi)
+        keep = 1.0 if turns >= fast else 0.0 if turns <= slow else (turns - slow) / (fast - slow)
+        seen.add(0 if turns <= slow else 2 if turns >= fast else 1)
+        assert abs(float(got[i]) - (keep * f + (1 - keep) * f / factor)) <= 1e-13 * f
+    assert seen == {0, 1, 2} and abs(mscale - (0.1 * math.log(factor) + 1)) < 1e-15
 
 
 def test_oracle_rounds_like_torch():
