@@ -933,6 +933,56 @@ def test_steps_of_a_layer_in_two_graphs():
         _check_out(o[:n], ref, weighted, size, d, 64)
 
 
+def test_rollbacks_over_page_ends_lose_no_page():
+    """Verify steps whose drafts are rejected in part, in one graph: the pages that a request no
+    longer reaches go back on the list on the device, and no page is lost or held twice."""
+    b, page, cols, draft, total = 6, 16, 40, 7, 200
+    st = {"ctx": _i32([3, 15, 16, 31, 40, 250]), "new": _i32([draft] * b), "keep": _i32([0] * b)}
+    store = torch.cat([torch.randperm(total, generator=_gen(1)).int(), torch.tensor([-1], dtype=torch.int32)]).to(DEV)
+    table, used = torch.full((b, cols), -1, dtype=torch.int32, device=DEV), _i32([0, 0, 0])
+
+    def give_back(had, keep, table, store, used, page):
+        first = (keep + page - 1) // page
+        gone = first < (had + page - 1) // page
+        at = first.clamp(max=table.shape[1] - 1).long()[:, None]
+        pages = table.gather(1, at)[:, 0]
+        gone &= pages >= 0
+        place = torch.where(gone, used[0] - gone.cumsum(0), store.numel() - 1)
+        store.scatter_(0, place, pages)
+        used[0] -= gone.sum()
+
+    def step():
+        r = ops.kv_slots(st["ctx"], st["new"], table, store[:-1], used, page, b * draft)
+        used.copy_(r.status)
+        st["ctx"].add_(st["keep"])  # of the draft, `keep` tokens are right
+        give_back(r.seq_lens, st["ctx"], table, store, used, page)
+        return r
+
+    zero = torch.zeros_like(st["ctx"])
+    r = ops.kv_slots(zero, st["ctx"], table, store[:-1], used, page, int(st["ctx"].sum()))
+    used.copy_(r.status)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step()  # keeps nothing: what it took goes back
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    rng = random.Random(2)
+    lens = st["ctx"].tolist()
+    for _ in range(40):
+        keep = [rng.randint(0, draft) for _ in range(b)]
+        st["keep"].copy_(_i32(keep))
+        graph.replay()
+        torch.cuda.synchronize()
+        lens = [n + k for n, k in zip(lens, keep)]
+        assert st["ctx"].tolist() == lens
+        n, rows = int(used[0]), table.tolist()
+        held = [p for row, ln in zip(rows, lens) for p in row[:-(-ln // page)]]
+        assert n == len(held) == sum(-(-ln // page) for ln in lens) and used.tolist()[1:] == [0, 0]
+        assert sorted(held + store[n:-1].tolist()) == list(range(total))
+
+
 # ---------------------------------------------------------------------------
 # refusals of the torch-facing calls
 # ---------------------------------------------------------------------------
