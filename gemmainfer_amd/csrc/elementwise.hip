@@ -192,11 +192,6 @@ int check_dtype(int dt, const char* who) {
   return GI_OK;
 }
 
-int after_launch(const char* what) {
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? GI_OK : hip_fail(e, what);
-}
-
 }  // namespace
 
 int launch_softcap(void* x, int dtype, int64_t n, float cap, hipStream_t stream) {
@@ -281,7 +276,7 @@ int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, con
   bool vec = D % 8 == 0 && rotary_dim % (interleaved ? 8 : 16) == 0;
   for (int w = 0; w < 2; ++w) {
     if (a.heads[w] == 0) continue;
-    vec = vec && ((uintptr_t)a.in[w] & 15) == 0 && ((uintptr_t)a.out[w] & 15) == 0;
+    vec = vec && aligned16(a.in[w]) && aligned16(a.out[w]);
     for (const int64_t s : {a.in_st[w], a.in_sh[w], a.out_st[w], a.out_sh[w]}) vec = vec && s * size % 16 == 0;
   }
   // dimensions that do not turn are left alone where the result takes the place of the input

@@ -13,6 +13,13 @@ namespace gi {
 // Sets the thread-local error message and returns `code`.
 int fail(int code, const std::string& msg);
 int hip_fail(hipError_t e, const char* what);
+// GI_OK (0), or the error that the launches before it left.
+inline int after_launch(const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : hip_fail(e, what);
+}
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Multiprocessor count of the current device (cached per device).
 int device_cu_count();
@@ -169,6 +176,12 @@ int launch_rope_rows(const void* q, void* q_out, const void* k, void* k_out, con
                      const int64_t* ko_strides, hipStream_t stream);
 
 // ---- 8-bit paged K/V cache (kv_cache.hip, kv_attention.hip) -------------------
+// log2 of a page's tokens (16, 32, 64, 128 or 256), or -1
+inline int log2_page(int page_size) {
+  for (int l = 4; l <= 8; ++l)
+    if (page_size == 1 << l) return l;
+  return -1;
+}
 int launch_kv_slots(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* block_table, int max_pages,
                     int64_t table_stride, const int32_t* free_pages, int n_free, const int32_t* free_used,
                     int page_size, int64_t* slots, int64_t* positions, int n_tokens, int32_t* q_start,

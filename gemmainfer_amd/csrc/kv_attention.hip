@@ -786,11 +786,6 @@ __global__ __launch_bounds__(kThreads) void kv_attention_join_kernel(AttnArgs a)
   }
 }
 
-int after_launch(const char* what) {
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? GI_OK : hip_fail(e, what);
-}
-
 // Tiles of 16 columns, by the mean columns of a request.
 int col_tiles(int T, int B, int G, int D) {
   const int64_t rows = ((int64_t)T * G + B - 1) / B;
@@ -894,9 +889,7 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
   if (T < 0 || B < 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || max_pages < 0 || table_stride < max_pages || num_pages < 0)
     return fail(GI_ERR_INVALID_ARG, "kv_attention: bad shape (Hq must be a multiple of Hk, table_stride >= max_pages)");
   if (!width_ok(D)) return fail(GI_ERR_UNSUPPORTED, "kv_attention: head widths 64, 128, 256 and 512");
-  int lp = -1;
-  for (int l = 4; l <= 8; ++l)
-    if (page_size == 1 << l) lp = l;
+  const int lp = log2_page(page_size);
   if (lp < 0) return fail(GI_ERR_INVALID_ARG, "kv_attention: page_size must be 16, 32, 64, 128 or 256");
   if (!q_start && T != B) return fail(GI_ERR_INVALID_ARG, "kv_attention: without q_start there is one row a request");
   if (Hk > kMaxGrid) return fail(GI_ERR_UNSUPPORTED, "kv_attention: at most 2^23 kv heads");
@@ -910,11 +903,11 @@ int launch_kv_attention(const void* q, int dtype, const int64_t* q_strides, cons
   if (!q || !k_cache || !v_cache || !k_scale || !v_scale || !seq_lens || !out || (max_pages > 0 && !block_table))
     return fail(GI_ERR_INVALID_ARG, "kv_attention: null pointer");
   for (const void* p : {q, k_cache, v_cache, (const void*)out})
-    if ((uintptr_t)p & 15) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
+    if (!aligned16(p)) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
   for (const int64_t s : {q_strides[0], q_strides[1], o_strides[0], o_strides[1]})
     if (s % 8) return fail(GI_ERR_INVALID_ARG, "kv_attention: row and head strides must be multiples of 8 elements");
   if (window >= (int64_t)max_pages * page_size) window = 0;  // no request is that long
-  if ((uintptr_t)workspace & 15) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
+  if (!aligned16(workspace)) return fail(GI_ERR_INVALID_ARG, "kv_attention: pointers must be 16-byte aligned");
   const Grid gr = grid_of(T, B, Hq, Hk, D, (int64_t)max_pages * page_size, col_tiles(T, B, Hq / Hk, D));
   if ((int64_t)gr.max_tiles * Hk > 0x7fffffff) return fail(GI_ERR_UNSUPPORTED, "kv_attention: too many rows");
   if (!workspace || workspace_bytes < part_bytes(gr, B, Hk, D))

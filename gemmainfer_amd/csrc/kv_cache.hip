@@ -437,19 +437,6 @@ __global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
   }
 }
 
-int after_launch(const char* what) {
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? GI_OK : hip_fail(e, what);
-}
-
-int log2_page(int page_size) {
-  for (int l = 4; l <= 8; ++l)
-    if (page_size == 1 << l) return l;
-  return -1;
-}
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
 }  // namespace
 
 int launch_kv_slots(const int32_t* ctx_lens, const int32_t* new_lens, int B, int32_t* block_table, int max_pages,
