@@ -46,7 +46,8 @@ COMMON_FLAGS = [
 # Flags of single files.  The attention kernels hold up to 256 accumulator
 # registers a lane beside the softmax's operands: with MFMAs that read and
 # write vector registers directly the compiler moves values to accumulation registers
-# only where it runs out (spills of the 64-column kernel: 407 -> 4).
+# only where it runs out (the 64-column kernel of width 256 spills 305 to
+# scratch in the default form, none in this one).
 FILE_FLAGS = {"kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 

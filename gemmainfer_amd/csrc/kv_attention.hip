@@ -10,12 +10,14 @@
 // product: tile column r is row r / G, head r % G, so K and V are read once for
 // all of them.
 //
-// Bound by HBM where rows are few (47 requests of 33 to 8190 tokens, 16 + 8 heads of
-// 256: 161 us, 4.9 TB/s; two of 70001 and 130005 tokens, 16 + 2 heads of 512: 80
-// us, 5.1 TB/s; a copy reaches 4.85), by issue where they are many (2048 rows on 8100 tokens:
-// 275 to 315 us by box, 860 to 750 TFLOP/s; matrix cores busy 35%, one wave a
-// SIMD), by the start and end of a round of workgroups between (9 requests of 7 rows
-// on 600 to 5000 tokens of width 512: 33 us, of which 17 without a unit).
+// Bound by memory where rows are few, and there by how evenly the items keep the chip
+// reading: 1024 requests of 2000 tokens, 16 + 8 heads of 256, read 5.7 TB/s (the call, 1484
+// us), 47 of 33 to 8190 tokens 4.9 (161 us), two of 70001 and 130005 tokens, 16 + 2 heads of
+// 512, 5.1 (80 us); a plain read reaches 6.6 to 6.8 over as many bytes.  Bound by issue
+// where rows are many (2048 rows on 8100 tokens: 263 to 312 us by box, 900 to 760 TFLOP/s;
+// matrix cores busy 37%, one wave a SIMD), by the start and end of a round of workgroups
+// between (9 requests of 7 rows on 600 to 5000 tokens of width 512: 34 us, of
+// which 17 without a unit).
 
 #include "../../include/gemmainfer_amd.h"
 #include "gi_common.h"
@@ -148,9 +150,9 @@ __device__ __forceinline__ int ceil_div(int n, int d) {
 // The chunk, in units: the tile units of a kv head go to `resident` workgroups
 // that the chip holds at a time, in k = 1 ... 4 rounds.  One round
 // is best where the chunks come out even (a few long requests: two of 70001 and 130005
-// tokens 77 us in one round, 91 in two), several where many requests of
-// other lengths leave workgroups idle (47 up to 8190 tokens: 214, 202 and 194 us in one,
-// two and three).  k is the one with the least estimate: rounds of whole
+// tokens 93 us with the join in one round, 112 in two), several where many requests of
+// other lengths leave workgroups idle (47 up to 8190 tokens: 186, 173, 173 and 175 us in
+// one to four).  k is the one with the least estimate: rounds of whole
 // chunks, or what any order of work stays under, and two units to start each round.
 // `sum` adds a number of each request up.
 template <typename Sum>
@@ -407,8 +409,9 @@ __global__ __launch_bounds__(kThreads, workgroups_per_cu(D, CT)) void kv_attenti
   constexpr int kParts = (size_t)RT * (D + 4) * kWaves * 4 <= 140000 ? 1 : 2;
   constexpr int DP = D / kParts, kPitch = DP + 4;
   // What may move over a step's loads: nothing, or where a compute unit holds
-  // two workgroups all that is no memory access (16 columns of 256: 186 us
-  // instead of 220, of 512 the other way 80.5 instead of 82.7, 64 of 256 278 instead of 294)
+  // two workgroups all that is no memory access (16 columns of 256: 173 us instead of
+  // 176; where it holds one, the other way: 64 columns of 256 268 instead of 357, 32 of
+  // 512 41 instead of 67)
   constexpr int kFree = workgroups_per_cu(D, CT) > 1 ? 0x8f : 0;
   constexpr size_t kRedBytes = (size_t)kWaves * RT * kPitch * 4, kQBytes = kQLds ? (size_t)CT * 2 * KS * kWave * 16 : 16;
   typedef typename Qk<F16>::frag frag;

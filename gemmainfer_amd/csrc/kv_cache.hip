@@ -32,10 +32,11 @@ namespace {
 // kv_slots
 // ---------------------------------------------------------------------------
 // One launch, no exchange between workgroups: each scans the B request lengths
-// into its own LDS (12 bytes of global reads a request) and then places its
-// 256 tokens (7 requests 3.4 us, 301 requests and 14,500 rows 5.5 us).  A fresh page j of a request starts at position j*P >= ctx, which
-// is one of the call's own tokens: that token's thread writes the table entry,
-// so table entries are never read and written in one call.  Bound by latency
+// into its own LDS (8 bytes of global reads a request) and then places its
+// 256 tokens (7 requests 3.4 us, 301 requests and 14,500 rows 5.5 us).  A fresh
+// page j of a request starts at position j*P >= ctx, which is one of the call's
+// own tokens: that token's thread writes the table entry, so table entries are
+// never read and written in one call.  Bound by latency
 // (lengths -> scan -> table entry -> slot).
 constexpr int kSlotThreads = 256;
 constexpr int kMaxRequests = 8192;  // two ints a request in LDS: 64 KB
@@ -246,13 +247,14 @@ __device__ __forceinline__ float page_scale(uint32_t amax_bits) {
 
 // One workgroup a (run of rows, head, K or V); a run is the rows of the call
 // that follow each other on one page, rows that are skipped between them or not,
-// and its first row's workgroup does it all: which row lands on each of the page's P places (the last one wins where
-// a slot is named twice), the largest value of those rows, the page's scale,
-// then the codes.  Everything of a page in one workgroup needs no atomics on
-// scales and no second launch.  A decode step is bound by latency (slots, then
-// rows and scale, then stores: 61 rows of 8 heads of 256 in 6 us), a prompt by its rows' two
-// reads (6000 rows: 27 us, 74 MB in and out; kept in registers instead, fewer workgroups fit and it
-// takes 34).  per_wg rows are looked at by one workgroup.
+// and its first row's workgroup does it all: which row lands on each of the
+// page's P places (the last one wins where a slot is named twice), the largest
+// value of those rows, the page's scale, then the codes.  Everything of a page in
+// one workgroup needs no atomics on scales and no second launch.  A decode step
+// is bound by latency (slots, then rows and scale, then stores: 61 rows of 8 heads
+// of 256 in 6 us), a prompt by its rows' two reads (6000 rows: 27 to 29 us, 74 MB
+// in and out; kept in registers instead, fewer workgroups fit and it takes 34).
+// per_wg rows are looked at by one workgroup.
 template <typename T, bool kVec>
 __global__ __launch_bounds__(kAppThreads) void kv_append_kernel(AppendArgs a) {
   __shared__ int last[kMaxPage];               // the row on each place, -1: none
@@ -492,11 +494,14 @@ int launch_kv_append(const void* k, const void* v, int dtype, const int64_t* k_s
   a.D = D;
   a.log_page = lp;
   // a decode step's rows lie on pages of their own: a workgroup each; a
-  // prompt's lie on its pages in runs, and most workgroups would find nothing
+  // prompt's lie on its pages in runs, and most workgroups would find nothing.
+  // The host sees only how many rows there are.  8 heads of 256, with 16, 4 and 1
+  // rows a workgroup: 1200 prompt rows 14, 18 and 32 us, 6000 28, 47 and 141; of
+  // lone rows 1040 48, 39 and 44, 2000 83, 67 and 79.
   a.per_wg = (int64_t)T * Hk > 8192 ? 16 : 1;
   // Of a prompt's workgroups every (page / 16)-th finds a run: in order, those
   // would all fall on a few of the chip's eight parts (6000 rows onto pages of
-  // 64: 29.8 us, spread out 27.7).
+  // 64: 29.7 us, spread out 28.5).
   const uint32_t blocks = (uint32_t)((T - 1) / a.per_wg + 1);
   a.blocks = blocks;
   a.spread = 1;

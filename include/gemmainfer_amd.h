@@ -420,7 +420,8 @@ int gi_kv_append(const void* k, const void* v, int dtype,
  * q, out bf16 or fp16 [T, Hq, D], last dimension contiguous, other strides
  * multiples of 8 elements, 16-byte aligned; D 64, 128, 256 or 512; fp32 sums
  * and softmax statistics.  Deterministic.  The workspace is scratch: it needs
- * no initial value and holds nothing between calls.  Its size depends on
+ * no initial value and holds nothing between calls.  It is not left zeroed, so
+ * it must be one of its own, not a workspace of the entries above.  Its size depends on
  * max_tokens = max_pages * page_size, what a row of the table has room for, and
  * does not shrink as T, B or max_tokens grow: a workspace for a program's largest
  * numbers serves its smaller calls on the same heads.                       */
