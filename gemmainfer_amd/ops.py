@@ -834,7 +834,8 @@ def kv_attention(q, cache: KVCache, block_table, seq_lens, q_start=None, *, scal
     tokens in the pages ``block_table[b]`` names, those rows' own among them.  A
     row sees the tokens up to its own, with ``window`` > 0 the last ``window`` of
     them; one that sees none gets zeros.  ``scale`` defaults to D ** -0.5.  Query
-    head h reads kv head h // (Hq // Hk).  Rows behind the last request are not
+    head h reads kv head h // (Hq // Hk).  ``out`` is like q, its rows contiguous
+    and 16-byte aligned, and overlaps neither what q spans nor itself.  Rows behind the last request are not
     computed: they keep what ``out`` holds, and are unspecified without it.  A
     row that sees a token without a page (one outside the cache) gets NaN, and so
     does every row of a request that is longer than its table."""
